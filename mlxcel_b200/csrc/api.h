@@ -173,6 +173,13 @@ long long mx_gemm_workspace_bytes(void);
 int mx_add_rmsnorm(const void* x, const void* residual, const void* weight, void* y,
                    void* residual_out, int rows, int dim, float eps, float w_bias, void* stream);
 
+// The step between two sub-layers (bf16, or fp32 where `fp32`; strides in elements):
+// h = residual + scale * gate * rms(x) * (post_w + w_bias), y = norm(h) * (pre_w + w_bias) + pre_b. NULL operands are left out (without
+// pre_w there is no y); layer_norm: the second norm is a layer norm. h may be x or residual itself.
+int mx_branch_norm(const void* x, long long ldx, const void* residual, long long ldr, const void* post_w, const void* gate,
+                   const void* pre_w, const void* pre_b, void* h, long long ldh, void* y, long long ldy, int rows, int dim,
+                   float scale, float eps, float w_bias, int layer_norm, int fp32, void* stream);
+
 // Per-head RMSNorm over the last dimension of [tokens, heads, head_dim] (Qwen3 q/k norm), in place.
 int mx_head_rmsnorm(void* x, const void* weight, int tokens, int heads, int head_dim,
                     long long token_stride, float eps, void* stream);
@@ -193,6 +200,25 @@ int mx_rope_append(void* qkv, const int* positions, const int* slot_mapping, con
                    const void* k_norm_w, float norm_eps, int T, int Hq, int Hkv, int D,
                    int rot_dim, int block_size, int rope_mode, float mscale, int kv_bits,
                    void* stream);
+
+// Rotary positions with several axes, and the append to the paged pool: frequency i turns with positions[axis[i] * ldp + t]. qkv
+// [T, (Hq + 2 Hkv) * D] bf16 with row stride ldqkv; rotated q goes to q_out (row stride ldq; q's own columns are fine), k and v into the
+// pool (layouts of mx_rope_append) at `slots`, those outside [0, n_slots) nowhere. pairs: columns (2i, 2i + 1) turn together, else
+// (i, i + rot_dim / 2). q_norm_w / k_norm_w: per-head rms norm before the rotation. mscale multiplies the rotated columns.
+int mx_mrope_append(const void* qkv, long long ldqkv, void* q_out, long long ldq, const int* positions, long long ldp, int axes,
+                    const int* axis, const int* slots, long long n_slots, const float* inv_freq, void* k_pool, void* v_pool,
+                    void* k_meta, void* v_meta, const void* q_norm_w, const void* k_norm_w, float norm_eps, int T, int Hq,
+                    int Hkv, int D, int rot_dim, int block_size, int pairs, float mscale, int kv_bits, void* stream);
+// q, k (rotated, pairs (i, i + D / 2)) and v of qkv [R, 3 * H * D] bf16 as fp32 [H, R, D].
+int mx_axial_rope(const void* qkv, long long ldqkv, float* q, float* k, float* v, const int* positions, long long ldp, int axes,
+                  const int* axis, const float* inv_freq, int R, int H, int D, void* stream);
+
+// Pages of a pool whose slab s starts at base[s] and has bytes[s] bytes per page (host arrays). job 0: copies by `table` = n pairs
+// (src, dst), then the first pairs of the `chains` chains and n (host/page_plan.cpp); 1: buffer <- the n pages of `table`; 2: the other
+// way. buffer: slab after slab, n pages each. table_dev: the table in device memory where it has more than mx_pages_inline_ints() ints.
+int mx_pages_inline_ints(void);
+int mx_pages(int job, const void* const* base, const long long* bytes, int n_slabs, void* buffer, const int* table,
+             const int* table_dev, int ints, int n, int chains, void* stream);
 
 // Paged decode attention (one query token per sequence), split-KV with an in-kernel merge.
 // q: rows of [Hq * D] bf16 with stride q_stride elements; out: [B, Hq * D] bf16.
@@ -246,6 +272,18 @@ int mx_sample(const void* logits, int logits_fp32, long long row_stride, const f
               const unsigned long long* steps, int* out_tokens, float* out_logprob, int B, int V,
               void* stream);
 long long mx_sample_scratch_floats(int B, int V);
+
+// Of every row of logits [R, V] (bf16 or fp32, row stride ld; the distribution is that of softcap * tanh((x + bias) * scale / softcap),
+// softcap 0: none): log probabilities of n_ids tokens ids[R, n_ids] (NaN outside the vocabulary), entropy, log normaliser, the `top`
+// most likely tokens (ties: lowest index) with their log probabilities. NaN logits count as -inf.
+int mx_token_logprobs(const void* logits, int fp32, long long ld, const void* ids, int ids64, int n_ids, const void* bias,
+                      int bias_fp32, float scale, float softcap, float* logprob, float* entropy, float* lse, int* top_ids,
+                      float* top_logprobs, int top, int R, int V, void* stream);
+// The same without alternatives for the logits x[M, K] @ w[V, K]^T (bf16, fp32 sums), which are not stored. partials: fp32
+// [3 * ceil(V / 256) + 1, M]; status: the device status word of bounded waits. -10: strides or addresses that TMA does not take.
+int mx_head_logprobs(const void* x, const void* w, const void* ids, int ids64, const void* bias, int bias_fp32, float scale,
+                     float softcap, float* partials, float* logprob, float* entropy, float* lse, int M, int V, int K, int ldx,
+                     int ldw, void* status, void* stream);
 
 // Repetition / frequency / presence penalties applied in place to fp32 or bf16 logits, given
 // per-row token histories [B, max_hist] (int32, -1 padded).

@@ -1,0 +1,223 @@
+// The step between two sub-layers of a residual stream, in one pass over the row:
+//
+//   b = rms(x) * (post_w + w_bias)          (post_w == NULL: b = x)
+//   h = round(residual + scale * gate * b)  (gate: a factor per channel)
+//   y = rms(h) * (pre_w + w_bias), or layer norm of h times (pre_w + w_bias) + pre_b
+//
+// Statistics, the branch and the sum are fp32. h is the stored residual stream, so it is rounded to the row type, and y is the norm
+// of the rounded row: what a later reader of the stream would compute. b and the scaled branch are not rounded in between.
+//
+// Bound by memory: x and residual in, h and y out, four rows. The row stays in registers between its reductions (two for rms, three
+// with the mean of a layer norm).
+#include "api.h"
+#include "common.cuh"
+#include "typed.cuh"
+
+namespace mx {
+
+struct BranchNormParams {
+  const void* x;
+  const void* residual;
+  const void* post_w;
+  const void* gate;
+  const void* pre_w;
+  const void* pre_b;
+  void* h;
+  void* y;
+  long long ldx, ldr, ldh, ldy;
+  int dim;
+  float scale, eps, w_bias;
+};
+
+// Sum over the CTA; `red` holds 32 floats that no other reduction in flight uses. One barrier: every thread adds the warps' sums.
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  const int warps = blockDim.x >> 5;
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float t = 0.f;
+  for (int i = 0; i < warps; ++i) t += red[i];
+  return t;
+}
+
+// V elements of type T in one access (16 bytes, or one element).
+template <typename T, int V>
+struct Pack {
+  static_assert(V == 1 || V * sizeof(T) == 16, "one element or 16 bytes");
+  uint4 w;
+  T e;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) e = *p;
+    else w = *reinterpret_cast<const uint4*>(p);
+  }
+  __device__ __forceinline__ void widen(float (&f)[V]) const {
+    if constexpr (V == 1) {
+      f[0] = to_f(e);
+    } else {
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (V == 8) f[2 * j] = bf16_lo(u[j]), f[2 * j + 1] = bf16_hi(u[j]);
+        else f[j] = __uint_as_float(u[j]);
+      }
+    }
+  }
+  // Rounds f to the type and leaves what is stored in f.
+  __device__ __forceinline__ void narrow(float (&f)[V]) {
+    if constexpr (V == 1) {
+      e = from_f<T>(f[0]);
+    } else if constexpr (V == 8) {
+      w = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    } else {
+      w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    widen(f);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (V == 1) *p = e;
+    else *reinterpret_cast<uint4*>(p) = w;
+  }
+};
+
+template <typename T, int V, int VPT, bool LAYER>
+__global__ void __launch_bounds__(1024) branch_norm_kernel(const BranchNormParams p) {
+  __shared__ float red[3][32];
+  pdl_trigger();
+  pdl_wait();
+  const size_t row = blockIdx.x;
+  const int nvec = p.dim / V;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+  const T* post = static_cast<const T*>(p.post_w);
+  const T* gate = static_cast<const T*>(p.gate);
+  const T* pre = static_cast<const T*>(p.pre_w);
+  const T* bias = static_cast<const T*>(p.pre_b);
+  Pack<T, V> xv[VPT], rv[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) {
+      xv[i].load(x + static_cast<size_t>(v) * V);
+      if (res) rv[i].load(res + static_cast<size_t>(v) * V);
+    }
+  }
+  float rstd = 1.f;
+  if (post) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (threadIdx.x + i * blockDim.x < nvec) {
+        float f[V];
+        xv[i].widen(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) ss += f[j] * f[j];
+      }
+    }
+    rstd = rsqrtf(row_sum(ss, red[0]) / static_cast<float>(p.dim) + p.eps);
+  }
+  float hv[VPT][V], stat = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) {
+      xv[i].widen(hv[i]);
+      Pack<T, V> t;
+      float f[V];
+      if (post) {
+        t.load(post + static_cast<size_t>(v) * V);
+        t.widen(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) hv[i][j] *= rstd * (f[j] + p.w_bias);
+      }
+      if (gate) {
+        t.load(gate + static_cast<size_t>(v) * V);
+        t.widen(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) hv[i][j] *= f[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) hv[i][j] *= p.scale;
+      if (res) {
+        rv[i].widen(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) hv[i][j] += f[j];
+      }
+      t.narrow(hv[i]);
+      t.store(static_cast<T*>(p.h) + row * p.ldh + static_cast<size_t>(v) * V);
+#pragma unroll
+      for (int j = 0; j < V; ++j) stat += LAYER ? hv[i][j] : hv[i][j] * hv[i][j];
+    }
+  }
+  if (pre == nullptr) return;
+  float mean = 0.f;
+  stat = row_sum(stat, red[1]) / static_cast<float>(p.dim);
+  if constexpr (LAYER) {                    // the variance from the centred row: no cancellation where the mean is large
+    mean = stat;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (threadIdx.x + i * blockDim.x < nvec) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) ss += (hv[i][j] - mean) * (hv[i][j] - mean);
+      }
+    }
+    stat = row_sum(ss, red[2]) / static_cast<float>(p.dim);
+  }
+  rstd = rsqrtf(stat + p.eps);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) {
+      Pack<T, V> t;
+      float f[V];
+      t.load(pre + static_cast<size_t>(v) * V);
+      t.widen(f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) hv[i][j] = (hv[i][j] - mean) * rstd * (f[j] + p.w_bias);
+      if (bias) {
+        t.load(bias + static_cast<size_t>(v) * V);
+        t.widen(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) hv[i][j] += f[j];
+      }
+      t.narrow(hv[i]);
+      t.store(static_cast<T*>(p.y) + row * p.ldy + static_cast<size_t>(v) * V);
+    }
+  }
+}
+
+template <typename T, int V, bool LAYER>
+static int launch_branch_norm(const BranchNormParams& p, int rows, cudaStream_t stream) {
+  const int nvec = p.dim / V;
+  int threads = (nvec + 31) / 32 * 32;
+  if (threads > 1024) threads = 1024;
+  const int vpt = (nvec + threads - 1) / threads;
+  cudaError_t e;
+  if (vpt <= 1) e = launch_kernel(branch_norm_kernel<T, V, 1, LAYER>, dim3(rows), dim3(threads), 0, stream, p);
+  else if (vpt <= 4) e = launch_kernel(branch_norm_kernel<T, V, 4, LAYER>, dim3(rows), dim3(threads), 0, stream, p);
+  else e = launch_kernel(branch_norm_kernel<T, V, 32 / V, LAYER>, dim3(rows), dim3(threads), 0, stream, p);
+  return static_cast<int>(e);
+}
+
+}  // namespace mx
+
+extern "C" int mx_branch_norm(const void* x, long long ldx, const void* residual, long long ldr, const void* post_w, const void* gate,
+                              const void* pre_w, const void* pre_b, void* h, long long ldh, void* y, long long ldy, int rows, int dim,
+                              float scale, float eps, float w_bias, int layer_norm, int fp32, void* stream_) {
+  using namespace mx;
+  if (rows <= 0) return 0;
+  if (dim <= 0 || dim > 32768 || x == nullptr || h == nullptr || (pre_w != nullptr && y == nullptr)) return -1;
+  const BranchNormParams p{x, residual, post_w, gate, pre_w, pre_b, h, y, ldx, ldr, ldh, ldy, dim, scale, eps, w_bias};
+  const int v = fp32 ? 4 : 8;
+  bool wide = dim % v == 0 && ldx % v == 0 && ldr % v == 0 && ldh % v == 0 && ldy % v == 0;
+  for (const void* a : {x, residual, post_w, gate, pre_w, pre_b, static_cast<const void*>(h), static_cast<const void*>(y)})
+    wide = wide && aligned_to(a, 16);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (fp32) {
+    if (wide) return layer_norm ? launch_branch_norm<float, 4, true>(p, rows, stream) : launch_branch_norm<float, 4, false>(p, rows, stream);
+    return layer_norm ? launch_branch_norm<float, 1, true>(p, rows, stream) : launch_branch_norm<float, 1, false>(p, rows, stream);
+  }
+  if (wide)
+    return layer_norm ? launch_branch_norm<__nv_bfloat16, 8, true>(p, rows, stream) : launch_branch_norm<__nv_bfloat16, 8, false>(p, rows, stream);
+  return layer_norm ? launch_branch_norm<__nv_bfloat16, 1, true>(p, rows, stream) : launch_branch_norm<__nv_bfloat16, 1, false>(p, rows, stream);
+}

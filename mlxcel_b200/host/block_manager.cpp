@@ -436,6 +436,7 @@ class BlockManager {
 }  // namespace
 
 void bind_scheduler(py::module_& m);
+void bind_page_plan(py::module_& m);
 
 PYBIND11_MODULE(_mlxcel_host, m) {
   m.doc() = "mlxcel_b200 host runtime (C++): KV block manager, prefix index, batch tables, tick policy";
@@ -468,4 +469,5 @@ PYBIND11_MODULE(_mlxcel_host, m) {
       .def("fill_slots", &BlockManager::fill_slots)
       .def("stats", &BlockManager::stats);
   bind_scheduler(m);
+  bind_page_plan(m);
 }

@@ -28,3 +28,5 @@ TickState = _host.TickState
 TickDecision = _host.TickDecision
 decide_tick = _host.decide_tick
 prefill_piece = _host.prefill_piece
+page_ids = _host.page_ids
+page_copies = _host.page_copies

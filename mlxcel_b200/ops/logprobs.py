@@ -1,0 +1,87 @@
+"""Log probabilities of given tokens, the entropy of every row's distribution and its most likely tokens, from logits
+(``csrc/logprobs.cu``) or straight from hidden rows and the head's weights."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib, linear, reference as ref
+
+MAX_TOP = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprob`` of the given tokens (shaped like them), ``entropy`` (nats) and log normaliser ``lse`` [R], ``top_ids`` int32 and
+    ``top_logprobs`` [R, top], most likely first and equal ones by index; all but the ids fp32."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def _check(rows: int, vocab: int, device, ids, bias, scale: float, softcap: float, dim: int) -> None:
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() not in (1, 2)[:dim] or ids.shape[0] != rows or ids.device != device:
+        raise ValueError(f"ids have to be int32 or int64 [{rows}]{f' or [{rows}, n]' if dim > 1 else ''} on {device}")
+    if bias is not None and (bias.shape != (vocab,) or bias.dtype not in (torch.bfloat16, torch.float32) or bias.device != device
+                             or not bias.is_contiguous()):
+        raise ValueError(f"bias has to be a contiguous bf16 or fp32 [{vocab}] tensor on {device}")
+    if not scale > 0.0 or not softcap >= 0.0:
+        raise ValueError("scale has to be positive and softcap not negative")
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, bias: torch.Tensor | None = None, scale: float = 1.0,
+                   softcap: float = 0.0) -> TokenLogprobs:
+    """``logits`` [R, V] (bf16 or fp32, rows may be strided) and the tokens asked for, ``ids`` [R] or [R, n]. The distribution is that
+    of ``softcap * tanh((logits + bias) * scale / softcap)`` (no cap: 0). NaN counts as -inf; a row with nothing left has log
+    probabilities and ``lse`` of -inf and entropy 0; an id outside the vocabulary has log probability NaN. ``top``: up to 64."""
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"logits have to be bf16 or fp32 [R, V], not {logits.dtype} {tuple(logits.shape)}")
+    R, V = logits.shape
+    _check(R, V, logits.device, ids, bias, scale, softcap, 2)
+    if not 0 <= top <= min(V, MAX_TOP) or V < 1:
+        raise ValueError(f"top {top} is not within 0 to {min(V, MAX_TOP)}")
+    if not logits.is_cuda:
+        return TokenLogprobs(*ref.token_logprobs(logits, ids, top, bias, scale, softcap))
+    if logits.stride(1) != 1 and V > 1 or R > 1 and logits.stride(0) < V:
+        raise ValueError("the logits of a row have to be adjacent and rows apart")
+    ids = ids.contiguous()
+    f = dict(dtype=torch.float32, device=logits.device)
+    r = TokenLogprobs(torch.empty(ids.shape, **f), torch.empty(R, **f), torch.empty(R, **f),
+                      torch.empty(R, top, dtype=torch.int32, device=logits.device), torch.empty(R, top, **f))
+    if R:
+        _lib.launch_on(logits.device, "mx_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
+                       int(ids.dtype == torch.int64), ids.numel() // R, _lib.ptr(bias), int(bias is not None and bias.dtype == torch.float32),
+                       float(scale), float(softcap), r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), r.top_ids.data_ptr(),
+                       r.top_logprobs.data_ptr(), top, R, V)
+    return r
+
+
+def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: torch.Tensor | None = None, scale: float = 1.0,
+                  softcap: float = 0.0) -> TokenLogprobs:
+    """:func:`token_logprobs` (without alternatives) of the logits ``x @ w^T``, which are fp32 and never rounded. ``x`` [R, K] and
+    the head's weights ``w`` [V, K] are bf16 (or both fp32); ``ids`` [R]."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
+        raise ValueError("hidden rows [R, K] and head weights [V, K] of one type are needed on one device")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"hidden rows have to be bf16 or fp32, not {x.dtype}")
+    R, V = x.shape[0], w.shape[0]
+    _check(R, V, x.device, ids, bias, scale, softcap, 1)
+    if V < 1 or x.shape[1] < 1:
+        raise ValueError("an empty vocabulary or width has no distribution")
+    if not x.is_cuda:
+        return TokenLogprobs(*ref.token_logprobs(x.float() @ w.float().t(), ids, 0, bias, scale, softcap))
+    if any(t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1] for t in (x, w)):
+        raise ValueError("the elements of a row have to be adjacent and rows apart")
+    f = dict(dtype=torch.float32, device=x.device)
+    r = TokenLogprobs(torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, 0, dtype=torch.int32, device=x.device),
+                      torch.empty(R, 0, **f))
+    part = max(1, (1 << 26) // V)                 # rows whose logits are held at once: 256 MB
+    with torch.cuda.device(x.device):
+        for r0 in range(0, R, part):
+            got = token_logprobs(linear(x[r0:r0 + part], w, out_fp32=True), ids[r0:r0 + part], bias=bias, scale=scale, softcap=softcap)
+            for whole, piece in zip(r[:3], got[:3]):
+                whole[r0:r0 + part] = piece
+    return r

@@ -1,0 +1,49 @@
+"""The step between two sub-layers of a residual stream as one operator: the norm behind a branch, its gate and scale, the sum with
+the residual and the norm in front of the next sub-layer (``csrc/branch_norm.cu``). Models with norms before and after each
+sub-layer, with scaled branches or with per-channel branch scales take it at every layer."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, reference as ref
+
+
+def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w: torch.Tensor | None = None,
+                gate: torch.Tensor | None = None, scale: float = 1.0, pre_w: torch.Tensor | None = None,
+                pre_b: torch.Tensor | None = None, layer_norm: bool = False, eps: float = 1e-6, w_bias: float = 0.0,
+                out: torch.Tensor | None = None) -> tuple[torch.Tensor | None, torch.Tensor]:
+    """``b = rmsnorm(x) * (post_w + w_bias)`` (``x`` itself without ``post_w``); ``h = residual + scale * gate * b``;
+    ``y = norm(h) * (pre_w + w_bias) + pre_b`` → ``(y, h)``, ``y`` None without ``pre_w``.
+
+    ``x`` and ``residual`` are [rows, dim] of one type (bf16 or fp32), their rows may be strided; ``gate`` (a factor per channel), the
+    weights and ``pre_b`` are [dim] of the same type. ``layer_norm``: the last norm is a layer norm (``pre_b`` belongs to it), else an
+    rms norm. Sums and statistics are fp32; ``h`` is rounded once and ``y`` is the norm of the rounded ``h``. ``out``: where ``h``
+    goes (``x`` or ``residual`` itself is fine)."""
+    if x.dim() != 2:
+        raise ValueError(f"branch_norm takes rows [rows, dim], not {tuple(x.shape)}")
+    rows, dim = x.shape
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"branch_norm takes bf16 or fp32 rows, not {x.dtype}")
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"{name} has to be like x: {tuple(x.shape)} {x.dtype} on {x.device}")
+    for name, t in (("post_w", post_w), ("gate", gate), ("pre_w", pre_w), ("pre_b", pre_b)):
+        if t is not None and (t.shape != (dim,) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous()):
+            raise ValueError(f"{name} has to be a contiguous [{dim}] {x.dtype} tensor on {x.device}")
+    if pre_b is not None and (pre_w is None or not layer_norm):
+        raise ValueError("pre_b belongs to a layer norm (pre_w, layer_norm=True)")
+    if dim < 1 or dim > 32768:
+        raise ValueError(f"rows of 1 to 32768 elements are covered, not {dim}")
+    if not x.is_cuda:
+        y, h = ref.branch_norm(x, residual, post_w, gate, scale, pre_w, pre_b, layer_norm, eps, w_bias)
+        return y, h if out is None else out.copy_(h)
+    for name, t in (("x", x), ("residual", residual), ("out", out)):
+        if t is not None and (t.stride(1) != 1 and dim > 1 or rows > 1 and t.stride(0) < dim):
+            raise ValueError(f"the elements of a row of {name} have to be adjacent and its rows apart")
+    h = torch.empty(rows, dim, dtype=x.dtype, device=x.device) if out is None else out
+    y = torch.empty(rows, dim, dtype=x.dtype, device=x.device) if pre_w is not None else None
+    if rows:
+        _lib.launch_on(x.device, "mx_branch_norm", x.data_ptr(), x.stride(0), _lib.ptr(residual), 0 if residual is None else residual.stride(0),
+                       _lib.ptr(post_w), _lib.ptr(gate), _lib.ptr(pre_w), _lib.ptr(pre_b), h.data_ptr(), h.stride(0), _lib.ptr(y), dim, rows, dim,
+                       float(scale), float(eps), float(w_bias), int(layer_norm), int(x.dtype == torch.float32))
+    return y, h

@@ -188,6 +188,107 @@ def apply_mrope(x: torch.Tensor, positions3: torch.Tensor, inv_freq: torch.Tenso
     return rot if rd == xf.shape[-1] else torch.cat([rot, xf[..., rd:]], dim=-1)
 
 
+def section_axes(sections, half: int, interleaved: bool = False) -> torch.Tensor:
+    """The axis (0 time, 1 height, 2 width) each of ``half`` frequencies turns with, int32: see :func:`apply_mrope`."""
+    if interleaved:
+        which = torch.zeros(half, dtype=torch.int32)
+        for comp in (1, 2):
+            which[comp:int(sections[comp]) * 3:3] = comp
+        return which
+    which = torch.repeat_interleave(torch.arange(len(sections), dtype=torch.int32) % 3, torch.tensor(list(sections)))[:half]
+    if which.numel() != half:
+        raise ValueError(f"sections {list(sections)} do not cover {half} frequencies")
+    return which
+
+
+def rotate_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, axes: torch.Tensor, rot_dim: int,
+                traditional: bool = False, mscale: float = 1.0) -> torch.Tensor:
+    """x [T, H, D] → fp32 with the first ``rot_dim`` columns of each head turned, frequency i by ``positions[axes[i]]``. Angles in
+    64 bits: an fp32 product of a far position is off by hundredths of a radian."""
+    half = rot_dim // 2
+    out = x.float().clone()
+    if half == 0:
+        return out
+    which = axes[:half].long().clamp(0, positions.shape[0] - 1)
+    ang = positions.double().t()[:, which] * inv_freq[:half].double()
+    cos, sin = ang.cos().float()[:, None], ang.sin().float()[:, None]
+    first, second = (slice(0, rot_dim, 2), slice(1, rot_dim, 2)) if traditional else (slice(0, half), slice(half, rot_dim))
+    a, b = out[..., first].clone(), out[..., second].clone()
+    out[..., first] = (a * cos - b * sin) * mscale
+    out[..., second] = (b * cos + a * sin) * mscale
+    return out
+
+
+def mrope_append(qkv, positions, slot_mapping, inv_freq, axes, kv, *, Hq, Hkv, D, rot_dim, traditional=False, mscale=1.0,
+                 q_norm_w=None, k_norm_w=None, norm_eps=1e-6) -> torch.Tensor:
+    """Plain statement of ``ops.rotary.mrope_append``."""
+    T = qkv.shape[0]
+    q, k, v = qkv.view(T, Hq + 2 * Hkv, D).float().split([Hq, Hkv, Hkv], 1)
+    norm = lambda t, w: t if w is None else t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + norm_eps) * w.float()    # noqa: E731
+    q = rotate_axes(norm(q, q_norm_w), positions, inv_freq, axes, rot_dim, traditional, mscale)
+    k = rotate_axes(norm(k, k_norm_w), positions, inv_freq, axes, rot_dim, traditional, mscale)
+    live = (slot_mapping >= 0) & (slot_mapping < kv.k.shape[0] * kv.block_size)
+    slots = slot_mapping[live].long()
+    at = (slots // kv.block_size, slice(None), slots % kv.block_size)
+    for pool, meta, new in ((kv.k, kv.k_meta, k[live]), (kv.v, kv.v_meta, v[live])):
+        if kv.kv_bits == 16:
+            pool[at] = new.to(pool.dtype)
+        else:
+            pool[at], meta[at] = (quantize_kv4 if kv.kv_bits == 4 else quantize_kv8)(new)
+    return q.to(qkv.dtype).reshape(T, Hq * D)
+
+
+def axial_rope(qkv, positions, inv_freq, axes, heads: int, D: int):
+    """Plain statement of ``ops.rotary.axial_rope``."""
+    x = qkv.view(qkv.shape[0], 3, heads, D)
+    turn = lambda t: rotate_axes(t, positions, inv_freq, axes, D).transpose(0, 1).contiguous()    # noqa: E731
+    return turn(x[:, 0]), turn(x[:, 1]), x[:, 2].float().transpose(0, 1).contiguous()
+
+
+def branch_norm(x, residual, post_w, gate, scale: float, pre_w, pre_b, layer_norm: bool, eps: float, w_bias: float):
+    """Plain statement of ``ops.norms.branch_norm``."""
+    b = x.float()
+    if post_w is not None:
+        b = b * torch.rsqrt(b.pow(2).mean(-1, keepdim=True) + eps) * (post_w.float() + w_bias)
+    if gate is not None:
+        b = b * gate.float()
+    b = b * scale
+    h = (b if residual is None else residual.float() + b).to(x.dtype)
+    if pre_w is None:
+        return None, h
+    z = h.float()
+    if layer_norm:
+        z = z - z.mean(-1, keepdim=True)
+    y = z * torch.rsqrt(z.pow(2).mean(-1, keepdim=True) + eps) * (pre_w.float() + w_bias)
+    return (y if pre_b is None else y + pre_b.float()).to(x.dtype), h
+
+
+def token_logprobs(logits, ids, top: int = 0, bias=None, scale: float = 1.0, softcap: float = 0.0):
+    """Plain statement of ``ops.logprobs.token_logprobs``: (logprob, entropy, lse, top_ids, top_logprobs)."""
+    z = logits.float()
+    if bias is not None:
+        z = z + bias.float()
+    z = z * scale
+    if softcap > 0:
+        z = softcap * torch.tanh(z / softcap)
+    z = torch.where(z.isnan(), torch.full_like(z, float("-inf")), z)
+    m = z.amax(-1, keepdim=True)
+    # a logit of +inf takes all the mass (shared with its equals); equal infinities are at distance 0
+    gap = torch.where(z == m, torch.zeros_like(z), z - m)
+    e = torch.where(z == float("-inf"), torch.zeros_like(z), gap.exp())
+    s = e.sum(-1)
+    log_s = s.log()
+    gone = s == 0
+    lse = torch.where(gone, torch.full_like(s, float("-inf")), m[:, 0] + log_s)
+    entropy = torch.where(gone, torch.zeros_like(s), log_s - torch.where(e > 0, e * gap, torch.zeros_like(e)).sum(-1) / s)
+    logp = torch.where(z == float("-inf"), z, gap - log_s[:, None])
+    V = z.shape[1]
+    i2 = (ids if ids.dim() == 2 else ids[:, None]).long()
+    logprob = torch.where((i2 < 0) | (i2 >= V), torch.full_like(i2, float("nan"), dtype=torch.float32), logp.gather(1, i2.clamp(0, V - 1)))
+    order = torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :top]
+    return logprob.view(ids.shape), entropy, lse, order.int(), logp.gather(1, order)
+
+
 def head_rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     xf = x.float()
     y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
