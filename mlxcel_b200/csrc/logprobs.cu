@@ -6,41 +6,12 @@
 // index. An id outside the vocabulary has log probability NaN.
 #include "api.h"
 #include "common.cuh"
+#include "logprobs.cuh"
 #include "typed.cuh"
 
 namespace mx {
 
 constexpr int kLpThreads = 512;
-constexpr float kLog2e = 1.4426950408889634f;
-
-// What a part of a row adds up to: the largest logit m, s = sum e^(z - m), t = sum e^(z - m) (z - m).
-struct LpSums {
-  float m, s, t;
-};
-// z - m where both may be infinite: equal infinities are at distance 0.
-__device__ __forceinline__ float lp_gap(float z, float m) { return z == m ? 0.f : z - m; }
-__device__ __forceinline__ LpSums lp_rescale(LpSums a, float m) {
-  const float d = lp_gap(a.m, m), e = exp2f(d * kLog2e);
-  if (e == 0.f) return {m, 0.f, 0.f};                                 // (d can be -inf, or s * d overflow)
-  return {m, a.s * e, (a.t + a.s * d) * e};
-}
-__device__ __forceinline__ LpSums lp_join(const LpSums& a, const LpSums& b) {
-  if (a.s == 0.f) return b;
-  if (b.s == 0.f) return a;
-  const float m = fmaxf(a.m, b.m);
-  const LpSums x = lp_rescale(a, m), y = lp_rescale(b, m);
-  return {m, x.s + y.s, x.t + y.t};
-}
-__device__ __forceinline__ LpSums lp_warp_join(LpSums a) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const LpSums b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)};
-    // (both lanes of a pair join in the same order, so that all lanes end with the same bits)
-    a = (threadIdx.x & o) ? lp_join(b, a) : lp_join(a, b);
-  }
-  return a;
-}
-
 struct LpParams {
   const void* logits;
   const void* ids;
@@ -56,13 +27,7 @@ struct LpParams {
 };
 
 // A logit as the row's distribution has it.
-__device__ __forceinline__ float lp_value(const LpParams& p, float x, int j) {
-  if (p.bias != nullptr) x += p.bias_fp32 ? static_cast<const float*>(p.bias)[j] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[j]);
-  x *= p.scale;
-  if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-  return x != x ? -INFINITY : x;
-}
-__device__ __forceinline__ float lp_log(float z, float m, float log_s) { return z == -INFINITY ? z : lp_gap(z, m) - log_s; }
+__device__ __forceinline__ float lp_value(const LpParams& p, float x, int j) { return lp_transform(x, j, p.bias, p.bias_fp32, p.scale, p.softcap); }
 
 // Orders by value, then by lower index; 0 is below every pair.
 __device__ __forceinline__ unsigned long long lp_key(float z, int j) {

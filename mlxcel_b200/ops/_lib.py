@@ -98,6 +98,7 @@ def _declare(lib) -> None:
                             _i, _f, _i, _vp],
         "mx_axial_rope": [_vp, _ll, _vp, _vp, _vp, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _vp],
         "mx_pages": [_i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp],
+        "mx_head_logprobs": [_vp, _vp, _vp, _i, _vp, _i, _f, _f, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
         "mx_token_logprobs": [_vp, _i, _ll, _vp, _i, _i, _vp, _i, _f, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
         "mx_add_rmsnorm": [_vp, _vp, _vp, _vp, _vp, _i, _i, _f, _f, _vp],
         "mx_head_rmsnorm": [_vp, _vp, _i, _i, _i, _ll, _f, _vp],

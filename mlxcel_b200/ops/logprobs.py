@@ -9,6 +9,7 @@ import torch
 from . import _lib, linear, reference as ref
 
 MAX_TOP = 64
+FUSED_ROWS = 256        # above, head_logprobs keeps its logits on the chip
 
 
 class TokenLogprobs(NamedTuple):
@@ -78,10 +79,19 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: 
     f = dict(dtype=torch.float32, device=x.device)
     r = TokenLogprobs(torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, 0, dtype=torch.int32, device=x.device),
                       torch.empty(R, 0, **f))
+    K = x.shape[1]
+    if R > FUSED_ROWS and x.dtype == torch.bfloat16 and not (K % 8 or x.stride(0) % 8 or w.stride(0) % 8 or (x.data_ptr() | w.data_ptr()) % 16):
+        partials = torch.empty(3 * (-(-V // 256)) + 1, R, **f)
+        ids = ids.contiguous()
+        _lib.launch_on(x.device, "mx_head_logprobs", x.data_ptr(), w.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), _lib.ptr(bias),
+                       int(bias is not None and bias.dtype == torch.float32), float(scale), float(softcap), partials.data_ptr(),
+                       r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), R, V, K, x.stride(0), w.stride(0),
+                       _lib.workspace(x.device).data_ptr())
+        return r
     part = max(1, (1 << 26) // V)                 # rows whose logits are held at once: 256 MB
     with torch.cuda.device(x.device):
         for r0 in range(0, R, part):
-            got = token_logprobs(linear(x[r0:r0 + part], w, out_fp32=True), ids[r0:r0 + part], bias=bias, scale=scale, softcap=softcap)
+            got = token_logprobs(linear(x[r0:r0 + part], w, out_fp32=True, w_fresh=True), ids[r0:r0 + part], bias=bias, scale=scale, softcap=softcap)
             for whole, piece in zip(r[:3], got[:3]):
                 whole[r0:r0 + part] = piece
     return r
