@@ -2,8 +2,8 @@
 // z = x[M, K] @ w[V, K]^T (+ bias), scaled and soft-capped, for each row lse = log sum e^z, log p(id) = z_id - lse, H = lse - sum p z.
 //
 // The products run as in gemm_pair.cu: 256 x 256 tiles on pairs of SMs, operands by TMA, accumulators in TMEM, double-buffered. The
-// epilogue leaves a tile as (m, s, t) of its 256 columns per row, m = max z, s = sum e^(z - m), t = sum e^(z - m) (z - m), in place
-// of 256 logits, and the row's own token's logit where the tile holds it. A second launch joins the column tiles of each row.
+// epilogue leaves a tile as the sums of its 256 columns per row (m, s, t of logprobs.cuh) in place of 256 logits, and the row's own
+// token's logit where the tile holds it. A second launch joins the column tiles of each row.
 // Logits of 2047 rows over 128256 tokens would be 1 GB of fp32; what is written instead is 12 MB. The logits are never rounded.
 //
 // Bound by the tensor cores: a tile's products take 8 K cycles an SM, its epilogue about 3400 beside them.
@@ -165,14 +165,19 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
           top = fmaxf(top, z[i]);
         }
         if (top > a.m) a = lp_rescale(a, top);
-        if (a.m != -INFINITY) {
+        if (lp_plain(a.m)) {
+          const float low = lp_floor(a.m);
+          lp_pair s2 = lp_two(a.s, 0.f), t2 = lp_two(a.t, 0.f);
+          float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            // where e^d is 0, d is kept finite: 0 * -inf is no number
-            const float d = fmaxf(lp_gap(z[i], a.m), -256.f), e = lp_exp2(d * kLog2e);
-            a.s += e;
-            a.t += e * d;
-          }
+          for (int i = 0; i < 32; ++i) f[i] = fmaxf(z[i], low);
+          lp_add(f, lp_two(-a.m, -a.m), s2, t2);
+          const float2 s = lp_both(s2), t = lp_both(t2);
+          a.s = s.x + s.y;
+          a.t = t.x + t.y;
+        } else if (a.m != -INFINITY) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) a.s += z[i] == a.m ? 1.f : 0.f;
         }
         if (own_col >= c && own_col < c + 32) {
 #pragma unroll
@@ -221,11 +226,10 @@ __global__ void __launch_bounds__(1024) head_join_kernel(const HeadParams p) {
   __syncthreads();
   if (warp != 0 || m >= p.M) return;
   for (int i = 1; i < 32; ++i) a = lp_join(a, {part[0][i][lane], part[1][i][lane], part[2][i][lane]});
-  const float log_s = logf(a.s);
   const long long id = head_id(p, m);
-  p.lse[m] = a.s > 0.f ? a.m + log_s : -INFINITY;
-  p.entropy[m] = a.s > 0.f ? log_s - a.t / a.s : 0.f;
-  p.logprob[m] = id < 0 || id >= p.V ? __int_as_float(0x7fc00000) : lp_log(p.partials[static_cast<size_t>(p.tiles_n) * 3 * p.M + m], a.m, log_s);
+  p.lse[m] = lp_lse(a);
+  p.entropy[m] = lp_entropy(a);
+  p.logprob[m] = id < 0 || id >= p.V ? __int_as_float(0x7fc00000) : lp_log(p.partials[static_cast<size_t>(p.tiles_n) * 3 * p.M + m], a);
 }
 
 }  // namespace mx

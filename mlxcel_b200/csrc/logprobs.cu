@@ -5,14 +5,23 @@
 // NaN counts as -inf. A row with nothing left (all -inf) has lse = -inf, log probabilities -inf and entropy 0. Equal logits order by
 // index. An id outside the vocabulary has log probability NaN.
 //
-// A row is read once, by a cluster of 1 to 8 CTAs (its parts are joined through distributed shared memory), as 16-byte vectors with
-// the next chunk in flight. Sums are per thread, rescaled at most once a chunk. The `top` best are found on the way: candidates
-// above a threshold go to a list in shared memory. The threshold is below the `top` best of what has been read: at first the best
-// but (top - 1) of 64 group maxima of a chunk (each group has an element at least that large), later the last of the list whenever
-// that is cut down to `top`. Lists are ordered by counting, for each entry, the entries above it. Every key is unique (value, then
-// index), so neither ties nor the order of arrival change a result.
+// A row is read by a cluster of 1 to 8 CTAs whose parts are joined through distributed shared memory, as 16-byte vectors that each
+// thread asks for two chunks ahead. Sums are per thread, rescaled at most once a chunk.
+//
+// The `top` best cost the pass over the row a maximum per thread and the chunk it came from. Behind it, each of 128 groups of threads
+// has an element at least as large as its maximum, so all of the `top` best are at or above the (top)th of these maxima, and only
+// groups whose own maximum is can hold one. Their vectors are read again (top 5 of 128 groups: 4 % of the row, top 20: 16 %), what
+// reaches the bound goes to a list, and the list is ordered by counting, for each entry, the entries above it. Every key is unique
+// (value, then index), so neither ties nor the order of arrival change a result. Should the list overflow (many of the largest logits a
+// whole number of rows of vectors apart), each of the `top` best is searched for. Looking for candidates on the way instead (against a
+// bound from the first chunk) cost more: every candidate sends its warp on a detour.
+//
+// Bound by memory, closely followed by the exponentials (16 a cycle and SM: 14.5 us for 509 x 128256, whose bf16 logits take 19.9 to
+// read) and the other 5 instructions per element, for which additions and products are done in pairs; all rows of such a call end at
+// the same time, so the way from the last logit to the result (joining, the search among groups) is not hidden. Measured, back to back
+// (us): 509 x 128256 bf16 31 without alternatives (24.6 without the exponentials), 45 with top 5, 53 with top 20; 512 x 151936 fp32 55
+// (floor 47), 80, 107; one row of 151936 fp32 5.5, 10.2, 12.9.
 #include <cooperative_groups.h>
-#include <string.h>
 
 #include <type_traits>
 
@@ -23,15 +32,28 @@
 
 namespace mx {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpVecs = 4;               // 16-byte vectors of a thread and chunk
+constexpr int kLpStages = 2;             // chunks of a thread in flight
 constexpr int kLpTop = 64;
-constexpr int kLpGroups = 64;            // of 4 neighbouring threads
-constexpr int kLpList = 2048;
-constexpr int kLpSlack = 32;             // entries of the list beyond twice those asked for before it is cut
+constexpr int kLpGroups = 128;           // of neighbouring threads
+constexpr int kLpList = 1088;            // at least kLpTop per CTA of a cluster, and the first vectors of kLpTop groups with the row's ends
 constexpr int kLpCluster = 8;
 using lp_key_t = unsigned long long;
+
+// The sums of a warp's lanes, the same bits in all of them: each is rescaled once, to the largest logit of all.
+__device__ __forceinline__ LpSums lp_warp_join(const LpSums& lane) {
+  float m = lane.s > 0.f ? lane.m : -INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  LpSums a = lane.s > 0.f ? lp_rescale(lane, m) : LpSums{m, 0.f, 0.f};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+  }
+  return a;
+}
+
 struct LpParams {
   const void* logits;
   const void* ids;
@@ -49,9 +71,9 @@ struct LpParams {
 // A logit as the row's distribution has it.
 __device__ __forceinline__ float lp_value(const LpParams& p, float x, int j) { return lp_transform(x, j, p.bias, p.bias_fp32, p.scale, p.softcap); }
 
-// Orders by value, then by lower index; 0 is below every pair.
+// Orders by value, then by lower index; NaN is -inf; 0 is below every key.
 __device__ __forceinline__ lp_key_t lp_key(float z, int j) {
-  uint32_t u = __float_as_uint(z + 0.f);                              // (-0 equals 0)
+  uint32_t u = __float_as_uint((z != z ? -INFINITY : z) + 0.f);       // (-0 equals 0)
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return (static_cast<lp_key_t>(u) << 32) | (0xffffffffu - static_cast<uint32_t>(j));
 }
@@ -61,24 +83,6 @@ __device__ __forceinline__ float lp_key_value(lp_key_t k) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-// A row's part: vectors [first, end) of 16 bytes, the first of them beginning `lead` elements before the row.
-template <typename T>
-struct LpPart {
-  static constexpr int E = 16 / sizeof(T);
-  const T* row;
-  int V, lead, first, end;
-  __device__ __forceinline__ int index(int v, int j) const { return v * E - lead + j; }
-  __device__ __forceinline__ uint4 load(int v) const {
-    const int j0 = index(v, 0);
-    if (j0 >= 0 && j0 + E <= V) return __ldg(reinterpret_cast<const uint4*>(row + j0));
-    T e[E];                                                            // the row's ends: what lies beyond is not read
-#pragma unroll
-    for (int j = 0; j < E; ++j) e[j] = j0 + j >= 0 && j0 + j < V ? row[j0 + j] : from_f<T>(-INFINITY);
-    uint4 u;
-    memcpy(&u, e, 16);
-    return u;
-  }
-};
 template <typename T>
 __device__ __forceinline__ void lp_unpack(const uint4& u, float (&f)[16 / sizeof(T)]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -88,285 +92,312 @@ __device__ __forceinline__ void lp_unpack(const uint4& u, float (&f)[16 / sizeof
     else f[i] = __uint_as_float(w[i]);
   }
 }
+__device__ __forceinline__ uint32_t lp_max2(uint32_t a, uint32_t b) {   // of two bf16 each; passes over NaN
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 struct LpNoLists {};
 struct LpLists {
   lp_key_t list[kLpList];
-  lp_key_t best[kLpTop];                   // this part's, in order (what the cluster reads)
   lp_key_t group[kLpGroups];
-  lp_key_t threshold;
-  int count[kLpWarps];
+  lp_key_t best[kLpTop];
+  lp_key_t bound;
+  int chosen[kLpTop];                      // groups that reach the bound
+  int n, groups;                           // entries that wanted into the list; chosen ones
 };
-
-// Entries of a[n] above `key`.
-__device__ __forceinline__ int lp_rank(const lp_key_t* a, int n, lp_key_t key) {
-  int r = 0;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) r += a[i] > key ? 1 : 0;
-  return r;
+// Calls take(i, how many of a[n] are above a[i]) for every entry but those that are 0, once. Up to 32 neighbouring threads count for
+// one entry. n <= kLpList; all threads of the CTA call it.
+template <int THREADS, typename F>
+__device__ __forceinline__ void lp_ranks(const lp_key_t* a, int n, F&& take) {
+  int share = 32;
+  while (share > 1 && share * n > THREADS) share >>= 1;
+  for (int i0 = 0; i0 < n; i0 += THREADS / share) {
+    const int i = i0 + threadIdx.x / share;
+    const lp_key_t key = i < n ? a[i] : ~0ull;
+    int r = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x % share; j < n; j += share) r += a[j] > key ? 1 : 0;
+    for (int o = share >> 1; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    if (i < n && key != 0 && threadIdx.x % share == 0) take(i, r);
+  }
 }
-// The `top` best of list[n] in order to best[] (0 where there are fewer). Ends with a barrier.
+__device__ __forceinline__ void lp_offer(LpLists& sh, lp_key_t key, lp_key_t bound) {
+  if (key >= bound) {
+    const int at = atomicAdd(&sh.n, 1);
+    if (at < kLpList) sh.list[at] = key;
+  }
+}
+// The `top` best of list[n], which is complete, in order to best[] (0 where there are fewer). Ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ void lp_select(LpLists& sh, int n, int top) {
-  for (int i = threadIdx.x; i < top; i += kLpThreads)
+  for (int i = threadIdx.x; i < top; i += THREADS)
     if (i >= n) sh.best[i] = 0;
-  for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const lp_key_t key = sh.list[i];
-    const int r = lp_rank(sh.list, n, key);
-    if (r < top) sh.best[r] = key;
-  }
+  lp_ranks<THREADS>(sh.list, n, [&](int i, int r) {
+    if (r < top) sh.best[r] = sh.list[i];
+  });
   __syncthreads();
 }
-// Places for `mine` entries of every thread behind each other: this thread's first, and the total. One barrier.
-__device__ __forceinline__ int lp_places(LpLists& sh, int mine, int& total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) sh.count[warp] = incl;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kLpWarps; ++i) {
-    if (i < warp) before += sh.count[i];
-    total += sh.count[i];
-  }
-  return before + incl - mine;
-}
-
-template <typename T, bool TOP, bool SHAPED>
-__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpParams p) {
-  constexpr int E = 16 / sizeof(T);
+template <typename T, bool TOP, bool SHAPED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LpParams p) {
+  constexpr int E = 16 / sizeof(T), kWarps = THREADS / 32, kStep = kLpVecs * THREADS;
+  constexpr bool kWhole = sizeof(T) == 2 && !SHAPED;                       // bf16 that needs no change: maxima without unpacking
+  extern __shared__ __align__(16) unsigned char lp_smem[];
+  uint4* ring = reinterpret_cast<uint4*>(lp_smem) + threadIdx.x;           // [stage][vector][thread]: a thread's own vectors on their way
   __shared__ std::conditional_t<TOP, LpLists, LpNoLists> sh;
-  __shared__ LpSums part_sums, warp_sums[kLpWarps];
+  __shared__ float warp_m[kWarps], warp_s[kWarps], warp_t[kWarps];
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   pdl_trigger();
   pdl_wait();
   const long long row = blockIdx.x / parts;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, top = p.top;
-  LpPart<T> x;
-  x.row = static_cast<const T*>(p.logits) + row * p.ld;
-  x.V = p.V;
-  x.lead = static_cast<int>(reinterpret_cast<uintptr_t>(x.row) % 16 / sizeof(T));
-  const int vecs = (p.V + x.lead + E - 1) / E, per = (vecs + parts - 1) / parts;
-  x.first = min(part * per, vecs);
-  x.end = min(x.first + per, vecs);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = static_cast<int>(threadIdx.x), top = p.top;
+  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  // `head` elements, then aligned vectors, then fewer than E elements
+  const int past = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)), head = min(past ? E - past : 0, p.V);
+  const int vecs = (p.V - head) / E, per = (vecs + parts - 1) / parts, first = min(part * per, vecs), end = min(first + per, vecs);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+
+  // A thread reads only what it asked for itself, so its own wait is all that is needed.
+  auto ask = [&](int v0, int stage) {
+#pragma unroll
+    for (int i = 0; i < kLpVecs; ++i) {
+      const int v = v0 + i * THREADS + tid;
+      if (v < end)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + (stage * kLpVecs + i) * THREADS)), "l"(xv + v) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kLpStages; ++i) ask(first + i * kStep, i);
 
   LpSums a{-INFINITY, 0.f, 0.f};
-  lp_key_t threshold = 0;
-  int listed = 0;
-  uint4 now[kLpVecs], next[kLpVecs];
-  auto fetch = [&](int v0, uint4 (&u)[kLpVecs]) {
-#pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) {
-      const int v = v0 + i * kLpThreads + threadIdx.x;
-      if (v < x.end) u[i] = x.load(v);
+  lp_key_t loose = 0;                                                     // of the row's ends
+  float peak = -INFINITY;                                                 // the thread's largest logit, and its chunk
+  int peak_at = first;
+  if (part == 0 && warp == 0) {                                           // the row's ends
+    const int tail = p.V - head - vecs * E, j = lane < head ? lane : vecs * E + lane;
+    if (lane < head + tail) {
+      const float z = lp_value(p, to_f(x[j]), j);
+      if (z != -INFINITY) a = {z, 1.f, 0.f};
+      loose = lp_key(z, j);
     }
-  };
-  auto values = [&](const uint4& u, int v, float (&f)[E]) {
-    lp_unpack<T>(u, f);
-    if constexpr (SHAPED) {
+  }
+  int stage = 0;
+  for (int v0 = first; v0 < end; v0 += kStep) {
+    uint4 now[kLpVecs];
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLpStages - 1) : "memory");
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int k = x.index(v, j);
-        f[j] = k >= 0 && k < x.V ? lp_value(p, f[j], k) : -INFINITY;
-      }
-    }
-  };
-  fetch(x.first, now);
-  for (int v0 = x.first; v0 < x.end; v0 += kLpVecs * kLpThreads) {
-    fetch(v0 + kLpVecs * kLpThreads, next);
-    float most = -INFINITY;
+    for (int i = 0; i < kLpVecs; ++i) now[i] = ring[(stage * kLpVecs + i) * THREADS];
+    const bool full = v0 + kStep <= end;
+    auto here = [&](int i) { return full || v0 + i * THREADS + tid < end; };
+    auto index = [&](int i, int j) { return head + (v0 + i * THREADS + tid) * E + j; };
+    auto values = [&](int i, float (&f)[E]) {
+      lp_unpack<T>(now[i], f);
+      if constexpr (SHAPED) {
 #pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) {
-      const int v = v0 + i * kLpThreads + threadIdx.x;
-      if (v < x.end) {
-        float f[E];
-        values(now[i], v, f);
-#pragma unroll
-        for (int j = 0; j < E; ++j) most = fmaxf(most, f[j]);           // (passes over NaN)
-      }
-    }
-    if (most > a.m) a = lp_rescale(a, most);
-    // e^d is 0 from d = -104 on: -256 stands for all that is lower, for masked values and (fmaxf drops it) for NaN
-    auto add = [&](auto&& gap) {
-#pragma unroll
-      for (int i = 0; i < kLpVecs; ++i) {
-        const int v = v0 + i * kLpThreads + threadIdx.x;
-        if (v < x.end) {
-          float f[E];
-          values(now[i], v, f);
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const float d = gap(f[j]), e = lp_exp2(d * kLog2e);
-            a.s += e;
-            a.t += e * d;
-          }
-        }
+        for (int j = 0; j < E; ++j) f[j] = lp_value(p, f[j], index(i, j));
       }
     };
-    if (a.m == INFINITY) add([](float z) { return z == INFINITY ? 0.f : -256.f; });
-    else if (a.m != -INFINITY) add([&](float z) { return fmaxf(z - a.m, -256.f); });
-    if constexpr (TOP) {
-      // what the threshold's value lets pass is looked at again as keys; NaN passes too and becomes -inf there
-      const float edge = threshold == 0 ? -INFINITY : lp_key_value(threshold);
-      const bool some = v0 + static_cast<int>(threadIdx.x) < x.end && most >= edge;
-      // the thread's elements above the threshold, in order of their index
-      auto each = [&](auto&& take) {
-        if (!some) return;
+    auto largest = [&](int i) {                                           // of vector i; passes over NaN
+      if constexpr (kWhole) {
+        const uint32_t w = lp_max2(lp_max2(now[i].x, now[i].y), lp_max2(now[i].z, now[i].w));
+        return fmaxf(fmaxf(bf16_lo(w), -INFINITY), bf16_hi(w));
+      } else {
+        float f[E], m = -INFINITY;
+        values(i, f);
 #pragma unroll
-        for (int i = 0; i < kLpVecs; ++i) {
-          const int v = v0 + i * kLpThreads + threadIdx.x;
-          if (v < x.end) {
-            float f[E];
-            values(now[i], v, f);
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-              if (!(f[j] < edge)) {
-                const int k = x.index(v, j);
-                const lp_key_t key = lp_key(f[j] != f[j] ? -INFINITY : f[j], k);
-                if (k >= 0 && k < x.V && key > threshold) take(key);
-              }
-            }
-          }
-        }
-      };
-      // the list's best stay, and the last of them is the threshold
-      auto cut = [&] {
-        lp_select(sh, listed, top);
-        listed = top;
-        if (sh.best[top - 1] > threshold) threshold = sh.best[top - 1];
-        for (int i = threadIdx.x; i < top; i += kLpThreads) sh.list[i] = sh.best[i];
-      };
-      const int threads = __syncthreads_count(some);
-      if (threads > kLpGroups) {                                          // many: raise the threshold by this chunk's group maxima
-        lp_key_t mine = 0;
-        each([&](lp_key_t key) { mine = key > mine ? key : mine; });
-#pragma unroll
-        for (int o = 1; o < kLpThreads / kLpGroups; o <<= 1) {
-          const lp_key_t other = __shfl_xor_sync(0xffffffffu, mine, o);
-          mine = other > mine ? other : mine;
-        }
-        if (threadIdx.x % (kLpThreads / kLpGroups) == 0) sh.group[threadIdx.x / (kLpThreads / kLpGroups)] = mine;
-        if (threadIdx.x == 0) sh.threshold = threshold;
-        __syncthreads();
-        if (threadIdx.x < kLpGroups) {
-          const lp_key_t key = sh.group[threadIdx.x];
-          // one below the key itself, which has to pass
-          if (key > threshold && lp_rank(sh.group, kLpGroups, key) == top - 1) sh.threshold = key - 1;
-        }
-        __syncthreads();
-        threshold = sh.threshold;
+        for (int j = 0; j < E; ++j) m = fmaxf(m, f[j]);
+        return m;
       }
-      if (threads > 0) {
-        int mine = 0, total;
-        each([&](lp_key_t) { ++mine; });
-        int at = lp_places(sh, mine, total);
-        if (listed + total > kLpList && listed > top) {                   // make room: the list's best stay
-          __syncthreads();
-          cut();
-          mine = 0;
-          each([&](lp_key_t) { ++mine; });
-          __syncthreads();
-          at = lp_places(sh, mine, total);
-        }
-        if (listed + total <= kLpList) {
-          at += listed;
-          each([&](lp_key_t key) { sh.list[at++] = key; });
-          listed += total;
-          if (listed > 2 * top + kLpSlack) {                              // a current threshold lets 1 / n of the list pass in the nth chunk
-            __syncthreads();
-            cut();
-          }
-        } else {
-          // still too many (large values side by side): one place of every thread's elements at a time
-          for (int step = 0; step < kLpVecs * E; ++step) {
-            lp_key_t held = 0;
+    };
+    float most = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < kLpVecs; ++i) {
-              const int v = v0 + i * kLpThreads + threadIdx.x;
-              if (v < x.end) {
-                float f[E];
-                values(now[i], v, f);
+    for (int i = 0; i < kLpVecs; ++i)
+      if (here(i)) most = fmaxf(most, largest(i));
+    // (every vector has been looked at: its place is free)
+    ask(v0 + kLpStages * kStep, stage);
+    stage = stage + 1 == kLpStages ? 0 : stage + 1;
+    if (most > a.m) a = lp_rescale(a, most);
+    if (lp_plain(a.m)) {
+      const float low = lp_floor(a.m);
+      const uint32_t low2 = pack_bf16(low, low);
+      const lp_pair minus_m = lp_two(-a.m, -a.m);
+      lp_pair s2 = lp_two(a.s, 0.f), t2 = lp_two(a.t, 0.f);
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                  const int k = x.index(v, j);
-                  if (i * E + j == step && k >= 0 && k < x.V) held = lp_key(f[j] != f[j] ? -INFINITY : f[j], k);
-                }
-              }
-            }
-            if (listed + kLpThreads > kLpList) {
-              __syncthreads();
-              cut();
-            }
-            const bool take = held > threshold;
-            __syncthreads();
-            at = lp_places(sh, take ? 1 : 0, total);
-            if (take) sh.list[listed + at] = held;
-            listed += total;
-            __syncthreads();
+      for (int i = 0; i < kLpVecs; ++i) {
+        if (here(i)) {
+          float f[E];
+          if constexpr (kWhole) {
+            lp_unpack<T>(make_uint4(lp_max2(now[i].x, low2), lp_max2(now[i].y, low2), lp_max2(now[i].z, low2), lp_max2(now[i].w, low2)), f);
+          } else {
+            values(i, f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) f[j] = fmaxf(f[j], low);
           }
+          lp_add(f, minus_m, s2, t2);
         }
-        __syncthreads();
+      }
+      const float2 s = lp_both(s2), t = lp_both(t2);
+      a.s = s.x + s.y;
+      a.t = t.x + t.y;
+    } else if (a.m != -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < kLpVecs; ++i) {
+        if (here(i)) {
+          float f[E];
+          values(i, f);
+#pragma unroll
+          for (int j = 0; j < E; ++j) a.s += f[j] == a.m ? 1.f : 0.f;
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) now[i] = next[i];
+    if (TOP && most > peak) peak = most, peak_at = v0;
   }
   a = lp_warp_join(a);
-  if (lane == 0) warp_sums[warp] = a;
-  __syncthreads();
-  a = warp_sums[0];
+  if (lane == 0) warp_m[warp] = a.m, warp_s[warp] = a.s, warp_t[warp] = a.t;
+  if constexpr (TOP) {
+    auto key_at = [&](const uint4& u, int v, int j) {                   // of element j of vector v
+      float f[E];
+      lp_unpack<T>(u, f);
+      const int k = head + v * E + j;
+      return lp_key(SHAPED ? lp_value(p, f[j], k) : f[j], k);
+    };
+    // the thread's largest key: in the first chunk with its largest value
+    constexpr int kGroup = THREADS / kLpGroups;
+    lp_key_t own = 0;
+    for (int i = 0; i < kLpVecs; ++i) {
+      const int v = peak_at + i * THREADS + tid;
+      if (v < end) {
+        const uint4 u = __ldg(xv + v);
 #pragma unroll
-  for (int i = 1; i < kLpWarps; ++i) a = lp_join(a, warp_sums[i]);
-  if constexpr (TOP) lp_select(sh, listed, top);
-  if (parts > 1) {
-    if (threadIdx.x == 0) part_sums = a;
-    cluster.sync();
-    if (part == 0) {
-      for (int i = 1; i < parts; ++i) a = lp_join(a, *cluster.map_shared_rank(&part_sums, i));
-      if constexpr (TOP) {
-        for (int i = threadIdx.x; i < parts * top; i += kLpThreads) sh.list[i] = cluster.map_shared_rank(sh.best, i / top)[i % top];
+        for (int j = 0; j < E; ++j) {
+          const lp_key_t k = key_at(u, v, j);
+          own = k > own ? k : own;
+        }
       }
     }
+#pragma unroll
+    for (int o = 1; o < kGroup; o <<= 1) {
+      const lp_key_t other = __shfl_xor_sync(0xffffffffu, own, o);
+      own = other > own ? other : own;
+    }
+    if (tid % kGroup == 0) sh.group[tid / kGroup] = own;
+    if (tid == 0) {
+      sh.bound = 0;
+      sh.n = 0;
+      sh.groups = 0;
+    }
+    __syncthreads();
+    lp_ranks<THREADS>(sh.group, kLpGroups, [&](int i, int r) {            // (keys are unique: so are the ranks)
+      if (r < top) {
+        sh.chosen[r] = i;
+        atomicMax(&sh.groups, r + 1);
+        if (r == top - 1) sh.bound = sh.group[i];
+      }
+    });
+    __syncthreads();
+    const lp_key_t bound = sh.bound;
+    const float edge = bound ? lp_key_value(bound) : -INFINITY;
+    if (loose) lp_offer(sh, loose, bound);
+    const int rows = (end - first + THREADS - 1) / THREADS, again = kGroup * sh.groups * rows;
+    for (int q = tid; q < again; q += THREADS) {
+      const int g = q / kGroup / rows, v = first + (q / kGroup - g * rows) * THREADS + sh.chosen[g] * kGroup + q % kGroup;
+      if (v < end) {
+        const uint4 u = __ldg(xv + v);
+        float f[E];
+        lp_unpack<T>(u, f);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (SHAPED || !(f[j] < edge)) lp_offer(sh, key_at(u, v, j), bound);       // (NaN passes and is -inf there)
+      }
+    }
+    __syncthreads();
+    if (sh.n <= kLpList) {
+      lp_select<THREADS>(sh, sh.n, top);
+    } else {
+      lp_key_t last = ~0ull;
+      for (int k = 0; k < top; ++k) {
+        own = loose < last ? loose : 0;
+        for (int v = first + tid; v < end; v += THREADS) {
+          const uint4 u = __ldg(xv + v);
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const lp_key_t c = key_at(u, v, j);
+            if (c < last && c > own) own = c;
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const lp_key_t c = __shfl_xor_sync(0xffffffffu, own, o);
+          if (c > own) own = c;
+        }
+        if (lane == 0) sh.group[warp] = own;
+        __syncthreads();
+        last = sh.group[0];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) last = sh.group[i] > last ? sh.group[i] : last;
+        if (tid == 0) sh.best[k] = last;
+        __syncthreads();
+      }
+    }
+  } else {
+    __syncthreads();
+  }
+  // every warp of part 0 joins the sums of all parts' warps (at most 64)
+  if (parts > 1) cluster.sync();
+  if (part == 0) {
+    a = {-INFINITY, 0.f, 0.f};
+    for (int i = lane; i < parts * kWarps; i += 32) {
+      const int from = i / kWarps, w = i % kWarps;
+      a = lp_join(a, {cluster.map_shared_rank(warp_m, from)[w], cluster.map_shared_rank(warp_s, from)[w], cluster.map_shared_rank(warp_t, from)[w]});
+    }
+    a = lp_warp_join(a);
+    if constexpr (TOP) {
+      if (parts > 1)
+        for (int i = tid; i < parts * top; i += THREADS) sh.list[i] = cluster.map_shared_rank(sh.best, i / top)[i % top];
+    }
+  }
+  if (parts > 1) {
     cluster.sync();                                                       // the other parts' memory has been read
     if (part != 0) return;
-    if constexpr (TOP) lp_select(sh, parts * top, top);
+    if constexpr (TOP) lp_select<THREADS>(sh, parts * top, top);
   }
-  const float log_s = logf(a.s);
-  if (threadIdx.x == 0) {
-    p.lse[row] = a.s > 0.f ? a.m + log_s : -INFINITY;
-    p.entropy[row] = a.s > 0.f ? log_s - a.t / a.s : 0.f;
+  if (tid == 0) {
+    p.lse[row] = lp_lse(a);
+    p.entropy[row] = lp_entropy(a);
   }
-  for (int i = threadIdx.x; i < p.n_ids; i += kLpThreads) {
+  for (int i = tid; i < p.n_ids; i += THREADS) {
     const long long id = p.ids64 ? static_cast<const long long*>(p.ids)[row * p.n_ids + i] : static_cast<const int*>(p.ids)[row * p.n_ids + i];
-    p.logprob[row * p.n_ids + i] =
-        id < 0 || id >= p.V ? __int_as_float(0x7fc00000) : lp_log(lp_value(p, to_f(x.row[id]), static_cast<int>(id)), a.m, log_s);
+    p.logprob[row * p.n_ids + i] = id < 0 || id >= p.V ? __int_as_float(0x7fc00000) : lp_log(lp_value(p, to_f(x[id]), static_cast<int>(id)), a);
   }
   if constexpr (TOP) {
-    for (int i = threadIdx.x; i < top; i += kLpThreads) {
+    for (int i = tid; i < top; i += THREADS) {
       p.top_ids[row * top + i] = lp_key_index(sh.best[i]);
-      p.top_logprobs[row * top + i] = lp_log(lp_key_value(sh.best[i]), a.m, log_s);
+      p.top_logprobs[row * top + i] = lp_log(lp_key_value(sh.best[i]), a);
     }
   }
 }
 
+// A row is cut while all CTAs still find an SM of their own, into parts of at least a chunk: with more CTAs the tails of the parts cost
+// more than the cut gives (74 rows of 128256 fp32, top 5: 16.5 us in 2 parts, 21.2 in 4; one row: 10.2 us in 8 parts, 22.9 in one).
 template <typename T, bool TOP>
 static cudaError_t launch_token_logprobs(const LpParams& p, int rows, cudaStream_t stream) {
-  const bool shaped = p.bias != nullptr || p.scale != 1.f || p.softcap > 0.f;
-  auto kern = shaped ? token_logprobs_kernel<T, TOP, true> : token_logprobs_kernel<T, TOP, false>;
-  // Four CTAs are resident on an SM: rows are cut until they fill the SMs, into parts of at least one chunk.
-  const long long slots = 4ll * device_sm_count(), chunk = static_cast<long long>(kLpVecs) * kLpThreads * 16 / sizeof(T);
+  constexpr int THREADS = 256, chunk = THREADS * kLpVecs * 16 / sizeof(T);
   int parts = 1;
-  while (parts < kLpCluster && 2ll * parts * rows <= slots && p.V > parts * chunk) parts *= 2;
+  while (parts < kLpCluster && 2ll * parts * rows <= device_sm_count() && p.V > static_cast<long long>(parts) * chunk) parts *= 2;
+  const bool shaped = p.bias != nullptr || p.scale != 1.f || p.softcap > 0.f;
+  auto kern = shaped ? token_logprobs_kernel<T, TOP, true, THREADS> : token_logprobs_kernel<T, TOP, false, THREADS>;
+  constexpr int bytes = kLpStages * kLpVecs * THREADS * 16;
+  static bool allowed[2][64] = {};
+  const cudaError_t e = allow_shared(kern, bytes, allowed[shaped]);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
