@@ -6,7 +6,7 @@
 //   mx_axial_rope    vision towers: q, k (rotated) and v of all heads as fp32 [H, R, D], what their attention reads
 //
 // An fp32 product of a position near 2^17 and its frequency is off by 2^-8 of a radian. The product and its reduction by whole turns
-// are therefore done in fp64 (64 of them per token, shared by all heads), sine and cosine of the remainder in fp32.
+// are therefore done in fp64 (64 of them per token, shared by all heads), sine and cosine of what is left of a turn in fp32.
 #include "api.h"
 #include "common.cuh"
 #include "typed.cuh"
@@ -27,9 +27,8 @@ struct MropeAngles {
 __device__ __forceinline__ void axis_angle(const MropeAngles& a, long long t, int i, float& sn, float& cs) {
   const int ax = min(max(a.axis[i], 0), a.axes - 1);
   const double ang = static_cast<double>(a.positions[ax * a.ldp + t]) * static_cast<double>(a.inv_freq[i]);
-  const double turns = rint(ang * 0.15915494309189535);                               // 1 / (2 pi)
-  const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, ang));     // 2 pi as a sum of two
-  sincosf(static_cast<float>(r), &sn, &cs);
+  const double turns = ang * 0.15915494309189535;                                     // 1 / (2 pi)
+  sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
 }
 
 struct MropeParams {
@@ -142,6 +141,151 @@ __global__ void __launch_bounds__(kMropeThreads) mrope_append_kernel(const Mrope
   }
 }
 
+// ----------------------------------------------------------------------------- heads as vectors
+// A lane holds 2 W columns of a head (W = 8 or 4, accesses of 16 or 8 bytes): the columns W u.. of the first half and their partners of
+// the second, or (pairs) 2 W neighbours; the lanes behind the rotated width copy 2 W neighbours. LPH lanes work on a head, those beyond
+// its D / (2 W) are idle. A CTA takes up to 4 tokens, so that its threads have an angle each; heads of all of them follow one another,
+// two of a thread's in flight.
+constexpr int kMropeTokens = 4;
+
+template <int W>
+struct MropeVec;
+template <>
+struct MropeVec<8> {
+  using type = uint4;
+  static __device__ __forceinline__ void widen(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = bf16_lo(w[i]), f[2 * i + 1] = bf16_hi(w[i]);
+  }
+  static __device__ __forceinline__ uint4 narrow(const float (&f)[8]) {
+    return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  }
+};
+template <>
+struct MropeVec<4> {
+  using type = uint2;
+  static __device__ __forceinline__ void widen(const uint2& v, float (&f)[4]) { f[0] = bf16_lo(v.x), f[1] = bf16_hi(v.x), f[2] = bf16_lo(v.y), f[3] = bf16_hi(v.y); }
+  static __device__ __forceinline__ uint2 narrow(const float (&f)[4]) { return make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])); }
+};
+
+// The first columns of a lane's two vectors, and whether they turn.
+template <int W>
+__device__ __forceinline__ bool unit_columns(int u, int half, int pairs, int& c0, int& c1) {
+  const bool turns = u * W < half;
+  if (pairs || !turns) {
+    c0 = 2 * W * u;                        // (behind the rotated width, 2 half columns, too)
+    c1 = c0 + W;
+  } else {
+    c0 = W * u;
+    c1 = half + W * u;
+  }
+  return turns;
+}
+// Turns a lane's 2 W values by the W angles from cs, sn on.
+template <int W>
+__device__ __forceinline__ void turn_unit(float (&a)[W], float (&b)[W], const float* cs, const float* sn, int pairs, float mscale) {
+  float c[W], s[W];
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + i);
+    *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(sn + i);
+  }
+  if (pairs) {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const float x0 = a[2 * i], y0 = a[2 * i + 1], x1 = b[2 * i], y1 = b[2 * i + 1];
+      a[2 * i] = (x0 * c[i] - y0 * s[i]) * mscale;
+      a[2 * i + 1] = (y0 * c[i] + x0 * s[i]) * mscale;
+      b[2 * i] = (x1 * c[W / 2 + i] - y1 * s[W / 2 + i]) * mscale;
+      b[2 * i + 1] = (y1 * c[W / 2 + i] + x1 * s[W / 2 + i]) * mscale;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = (x * c[i] - y * s[i]) * mscale;
+      b[i] = (y * c[i] + x * s[i]) * mscale;
+    }
+  }
+}
+
+template <int W, int LPH, bool NORM>
+__global__ void __launch_bounds__(kMropeThreads, 4) mrope_append_vec_kernel(const MropeParams p, int tokens, int per_block) {
+  using Vec = typename MropeVec<W>::type;
+  __shared__ __align__(16) float cs[kMropeTokens * kMropeMaxDim / 2], sn[kMropeTokens * kMropeMaxDim / 2];
+  constexpr int HPI = kMropeThreads / LPH;
+  pdl_trigger();
+  pdl_wait();
+  const int t0 = blockIdx.x * per_block, rows = min(per_block, tokens - t0), heads = p.Hq + 2 * p.Hkv, half = p.ang.half, D = p.D;
+  const int g = threadIdx.x / LPH, u = threadIdx.x % LPH, items = rows * heads;
+  int c0, c1;
+  const bool turns = unit_columns<W>(u, half, p.pairs, c0, c1), live = u * 2 * W < D;
+  Vec v[2][2];
+  auto load = [&](int item, Vec (&x)[2]) {
+    if (live && item < items) {
+      const int t = item / heads;
+      const __nv_bfloat16* src = p.qkv + (t0 + t) * p.ldqkv + static_cast<long long>(item - t * heads) * D;
+      x[0] = *reinterpret_cast<const Vec*>(src + c0);
+      x[1] = *reinterpret_cast<const Vec*>(src + c1);
+    }
+  };
+  load(g, v[0]);
+  load(g + HPI, v[1]);
+  for (int i = threadIdx.x; i < rows * half; i += kMropeThreads) {
+    const int t = i / half;
+    axis_angle(p.ang, t0 + t, i - t * half, sn[i], cs[i]);
+  }
+  __syncthreads();
+  // whole warps stay in the loop: the norm's sums are exchanged between lanes
+  for (int first = g - g % (32 / LPH > 0 ? 32 / LPH : 1), item = g, k = 0; first < items; first += HPI, item += HPI, k ^= 1) {
+    float a[W], b[W];
+    const bool here = live && item < items;
+    const int t = item / heads, s = item - t * heads;
+    const bool is_q = s < p.Hq, is_v = s >= p.Hq + p.Hkv;
+    if (here) {
+      MropeVec<W>::widen(k ? v[1][0] : v[0][0], a);
+      MropeVec<W>::widen(k ? v[1][1] : v[0][1], b);
+    }
+    if (k) load(item + 2 * HPI, v[1]);
+    else load(item + 2 * HPI, v[0]);
+    if constexpr (NORM) {
+      float ss = 0.f;
+      if (here) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) ss += a[i] * a[i] + b[i] * b[i];
+      }
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const __nv_bfloat16* nw = is_q ? p.q_norm_w : (is_v ? nullptr : p.k_norm_w);
+      if (here && nw != nullptr) {                              // (not rounded before the rotation)
+        const float rstd = rsqrtf(ss / D + p.eps);
+        float w[W];
+        MropeVec<W>::widen(*reinterpret_cast<const Vec*>(nw + c0), w);
+#pragma unroll
+        for (int i = 0; i < W; ++i) a[i] *= rstd * w[i];
+        MropeVec<W>::widen(*reinterpret_cast<const Vec*>(nw + c1), w);
+#pragma unroll
+        for (int i = 0; i < W; ++i) b[i] *= rstd * w[i];
+      }
+    }
+    if (!here) continue;
+    if (turns && !is_v) turn_unit<W>(a, b, cs + t * half + W * u, sn + t * half + W * u, p.pairs, p.mscale);
+    __nv_bfloat16* dst;
+    if (is_q) {
+      dst = p.q_out + (t0 + t) * p.ldq + static_cast<long long>(s) * D;
+    } else {
+      const long long slot = p.slots[t0 + t];
+      if (slot < 0 || slot >= p.n_slots) continue;              // a row without a slot leaves the pool alone
+      const long long blk = slot / p.block_size;
+      const int head = s - p.Hq - (is_v ? p.Hkv : 0);
+      dst = static_cast<__nv_bfloat16*>(is_v ? p.v_pool : p.k_pool) + ((blk * p.Hkv + head) * p.block_size + (slot - blk * p.block_size)) * D;
+    }
+    *reinterpret_cast<Vec*>(dst + c0) = MropeVec<W>::narrow(a);
+    *reinterpret_cast<Vec*>(dst + c1) = MropeVec<W>::narrow(b);
+  }
+}
+
 struct AxialParams {
   const __nv_bfloat16* qkv;
   float* q;
@@ -175,6 +319,71 @@ __global__ void __launch_bounds__(kMropeThreads) axial_rope_kernel(const AxialPa
   }
 }
 
+template <int W, int LPH>
+__global__ void __launch_bounds__(kMropeThreads, 4) axial_rope_vec_kernel(const AxialParams p, int per_block) {
+  using Vec = typename MropeVec<W>::type;
+  __shared__ __align__(16) float cs[kMropeTokens * kMropeMaxDim / 2], sn[kMropeTokens * kMropeMaxDim / 2];
+  constexpr int HPI = kMropeThreads / LPH;
+  pdl_trigger();
+  pdl_wait();
+  const long long t0 = static_cast<long long>(blockIdx.x) * per_block;
+  const int rows = static_cast<int>(min(static_cast<long long>(per_block), p.rows - t0)), half = p.ang.half, D = p.D;
+  const int g = threadIdx.x / LPH, u = threadIdx.x % LPH, items = rows * 3 * p.H;
+  int c0, c1;
+  unit_columns<W>(u, half, 0, c0, c1);
+  const bool live = u * 2 * W < D;
+  // neighbouring groups take neighbouring rows of one head: their results are adjacent
+  auto place = [&](int item, int& t, int& h) {
+    h = item / rows;                                            // q of all heads, k, v
+    t = item - h * rows;
+  };
+  Vec v[2][2];
+  auto load = [&](int item, Vec (&x)[2]) {
+    if (live && item < items) {
+      int t, h;
+      place(item, t, h);
+      const __nv_bfloat16* src = p.qkv + (t0 + t) * p.ldqkv + static_cast<long long>(h) * D;
+      x[0] = *reinterpret_cast<const Vec*>(src + c0);
+      x[1] = *reinterpret_cast<const Vec*>(src + c1);
+    }
+  };
+  load(g, v[0]);
+  load(g + HPI, v[1]);
+  for (int i = threadIdx.x; i < rows * half; i += kMropeThreads) axis_angle(p.ang, t0 + i / half, i % half, sn[i], cs[i]);
+  __syncthreads();
+  if (!live) return;
+  for (int item = g, k = 0; item < items; item += HPI, k ^= 1) {
+    float a[W], b[W];
+    MropeVec<W>::widen(k ? v[1][0] : v[0][0], a);
+    MropeVec<W>::widen(k ? v[1][1] : v[0][1], b);
+    if (k) load(item + 2 * HPI, v[1]);
+    else load(item + 2 * HPI, v[0]);
+    int t, h;
+    place(item, t, h);
+    const int part = h / p.H;
+    if (part < 2) turn_unit<W>(a, b, cs + t * half + W * u, sn + t * half + W * u, 0, 1.f);
+    float* dst = (part == 0 ? p.q : part == 1 ? p.k : p.v) + (static_cast<long long>(h - part * p.H) * p.rows + t0 + t) * D;
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      *reinterpret_cast<float4*>(dst + c0 + i) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+      *reinterpret_cast<float4*>(dst + c1 + i) = make_float4(b[i], b[i + 1], b[i + 2], b[i + 3]);
+    }
+  }
+}
+
+// Tokens of a CTA: as many as have an angle per thread, while every SM still gets four CTAs.
+static int mrope_tokens(int T) {
+  int n = kMropeTokens;
+  while (n > 1 && T < 4 * n * device_sm_count()) n /= 2;
+  return n;
+}
+// Columns per access (8, 4; 0: not in vectors) for heads of D whose first rot columns turn.
+static int mrope_width(int D, int rot, uintptr_t addresses, long long strides) {
+  for (int w : {8, 4})
+    if (rot > 0 && D % (2 * w) == 0 && rot % (2 * w) == 0 && strides % w == 0 && addresses % (2 * w) == 0) return w;
+  return 0;
+}
+
 }  // namespace mx
 
 extern "C" int mx_mrope_append(const void* qkv, long long ldqkv, void* q_out, long long ldq, const int* positions, long long ldp, int axes,
@@ -198,6 +407,24 @@ extern "C" int mx_mrope_append(const void* qkv, long long ldqkv, void* q_out, lo
   p.eps = norm_eps, p.mscale = mscale;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   cudaError_t e;
+  auto bits_of = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
+  const int w = kv_bits == 16 ? mrope_width(D, rot_dim, bits_of(qkv) | bits_of(q_out) | bits_of(k_pool) | bits_of(v_pool) | bits_of(q_norm_w) | bits_of(k_norm_w),
+                                            ldqkv | ldq) : 0;
+  if (w != 0) {
+    const int lanes = D / (2 * w), per = mrope_tokens(T), blocks = (T + per - 1) / per;
+    const bool norm = q_norm_w != nullptr || k_norm_w != nullptr;
+#define MX_MROPE(W_, L_)                                                                                                          \
+    e = norm ? launch_kernel(mrope_append_vec_kernel<W_, L_, true>, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)      \
+             : launch_kernel(mrope_append_vec_kernel<W_, L_, false>, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)
+    if (w == 8 && lanes <= 4) MX_MROPE(8, 4);
+    else if (w == 8 && lanes <= 8) MX_MROPE(8, 8);
+    else if (w == 8) MX_MROPE(8, 16);
+    else if (lanes <= 8) MX_MROPE(4, 8);
+    else if (lanes <= 16) MX_MROPE(4, 16);
+    else MX_MROPE(4, 32);
+#undef MX_MROPE
+    return static_cast<int>(e);
+  }
   if (kv_bits == 16) e = launch_kernel(mrope_append_kernel<16>, dim3(T), dim3(kMropeThreads), 0, stream, p);
   else if (kv_bits == 8) e = launch_kernel(mrope_append_kernel<8>, dim3(T), dim3(kMropeThreads), 0, stream, p);
   else e = launch_kernel(mrope_append_kernel<4>, dim3(T), dim3(kMropeThreads), 0, stream, p);
@@ -210,5 +437,14 @@ extern "C" int mx_axial_rope(const void* qkv, long long ldqkv, float* q, float* 
   if (R <= 0 || H <= 0) return 0;
   if (D <= 0 || D > kMropeMaxDim || D % 2 || axes < 1) return -1;
   AxialParams p{static_cast<const __nv_bfloat16*>(qkv), q, k, v, {positions, axis, inv_freq, ldp, axes, D / 2}, ldqkv, R, H, D};
+  const int w = mrope_width(D, D, reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v),
+                            ldqkv);
+  if (w != 0) {
+    const int lanes = D / (2 * w), per = mrope_tokens(R), blocks = (R + per - 1) / per;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    auto run = [&](auto kern) { return static_cast<int>(launch_kernel(kern, dim3(blocks), dim3(kMropeThreads), 0, stream, p, per)); };
+    if (w == 8) return lanes <= 4 ? run(axial_rope_vec_kernel<8, 4>) : lanes <= 8 ? run(axial_rope_vec_kernel<8, 8>) : run(axial_rope_vec_kernel<8, 16>);
+    return lanes <= 8 ? run(axial_rope_vec_kernel<4, 8>) : lanes <= 16 ? run(axial_rope_vec_kernel<4, 16>) : run(axial_rope_vec_kernel<4, 32>);
+  }
   return static_cast<int>(launch_kernel(axial_rope_kernel, dim3(R), dim3(kMropeThreads), 0, static_cast<cudaStream_t>(stream_), p));
 }
