@@ -22,7 +22,9 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import KVLayer
+from ..ops.pages import PageSlabs
 
+STAGING_BYTES = 256 << 20                  # of blocks on their way between the pool and the host
 SLABS = ("k", "v", "k_meta", "v_meta", "k_mean", "v_mean")
 
 
@@ -37,6 +39,7 @@ class KVPool:
         L = cfg.num_hidden_layers if num_layers is None else num_layers
         shape = (num_blocks, self.Hkv, block_size, self.D)
         self.layers: list[KVLayer] = []
+        self._page_slabs = None
         geo = cfg.kv_geometry()
         if geo is not None:
             # one slab pair per attention run, each with its own head count and key / value widths
@@ -99,28 +102,59 @@ class KVPool:
             per_tok += Hkv * (cfg.head_dim // 64) * 4
         return 2 * per_tok * block_size * L
 
+    def _slab_names(self) -> list[tuple[int, str]]:
+        return [(i, n) for i, l in enumerate(self.layers) for n in SLABS if getattr(l, n) is not None]
+
+    def page_slabs(self) -> PageSlabs:
+        """The pool's slabs as :class:`~mlxcel_b200.ops.pages.PageSlabs`, in the order of their layers."""
+        slabs = [getattr(self.layers[i], n) for i, n in self._slab_names()]
+        h = self._page_slabs
+        if h is None or len(h[0]) != len(slabs) or any(a is not b for a, b in zip(h[0], slabs)):
+            h = self._page_slabs = (slabs, PageSlabs(slabs))
+        return h[1]
+
     def copy_blocks(self, pairs: list[tuple[int, int]]) -> None:
-        """Copy-on-write support: duplicate block contents ``src -> dst`` in every layer."""
-        if not pairs:
-            return
-        src = torch.tensor([p[0] for p in pairs], device=self.layers[0].k.device)
-        dst = torch.tensor([p[1] for p in pairs], device=self.layers[0].k.device)
-        for l in self.layers:
-            for n in SLABS:
-                t = getattr(l, n)
-                if t is not None:
-                    t[dst] = t[src]
+        """Copies block contents ``src -> dst`` in every layer (copy-on-write, forks, compaction): every block named as a destination,
+        once, becomes what its source was before the call, also where blocks are both."""
+        if pairs:
+            self.page_slabs().copy([p[0] for p in pairs], [p[1] for p in pairs])
+
+    def _batches(self, count: int):
+        """Runs of slabs (first, end) whose ``count`` blocks fit the staging buffer."""
+        sizes, first = self.page_slabs().page_bytes, 0
+        while first < len(sizes):
+            end, total = first + 1, sizes[first] * count
+            while end < len(sizes) and total + sizes[end] * count <= STAGING_BYTES:
+                total += sizes[end] * count
+                end += 1
+            yield first, end
+            first = end
 
     def extract_blocks(self, block_ids: list[int]) -> list[dict]:
         """Host copies of blocks (KV handoff / snapshot)."""
-        idx = torch.tensor(block_ids, device=self.layers[0].k.device)
-        out = []
-        for l in self.layers:
-            out.append({n: getattr(l, n)[idx].cpu() for n in SLABS if getattr(l, n) is not None})
+        slabs, n = self.page_slabs(), len(block_ids)
+        flat: list[torch.Tensor] = []
+        for first, end in self._batches(n):
+            data, at = slabs.gather(block_ids, first=first, count=end - first).cpu(), 0
+            for t, size in zip(slabs.slabs[first:end], slabs.page_bytes[first:end]):
+                flat.append(data[at:at + size * n].view(t.dtype).view(n, *t.shape[1:]))
+                at += size * n
+        out: list[dict] = [{} for _ in self.layers]
+        it = iter(flat)
+        for i, name in self._slab_names():
+            t = getattr(self.layers[i], name)
+            out[i][name] = next(it) if t.numel() else torch.zeros((n, *t.shape[1:]), dtype=t.dtype)
         return out
 
     def restore_blocks(self, block_ids: list[int], data: list[dict]) -> None:
-        idx = torch.tensor(block_ids, device=self.layers[0].k.device)
-        for l, d in zip(self.layers, data):
-            for n, t in d.items():
-                getattr(l, n)[idx] = t.to(getattr(l, n).device)
+        """Puts what :meth:`extract_blocks` returned into blocks, each named once."""
+        slabs, n = self.page_slabs(), len(block_ids)
+        if n == 0:
+            return
+        rows = [data[i][name] for i, name in self._slab_names() if getattr(self.layers[i], name).numel()]
+        for first, end in self._batches(n):
+            buf, at = torch.empty(n * sum(slabs.page_bytes[first:end]), dtype=torch.uint8, device=slabs.device), 0
+            for t, size, src in zip(slabs.slabs[first:end], slabs.page_bytes[first:end], rows[first:end]):
+                buf[at:at + size * n].view(t.dtype).view(n, *t.shape[1:]).copy_(src)
+                at += size * n
+            slabs.scatter(block_ids, buf, first=first, count=end - first)
