@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import ops
-from ..ops import recurrent as rops
+from ..ops import norms, recurrent as rops
 
 
 class Dinov2Backbone:
@@ -92,14 +92,13 @@ class Dinov2Backbone:
                 y = rops.layernorm(h, *self.final_ln, self.eps) if self.apply_ln else h
                 outs.append(y.view(N, T, hid))
         emit(0)
+        y = rops.layernorm(h, *self.blocks[0]["n1"], self.eps) if self.blocks else None
         for li, b in enumerate(self.blocks):
-            y = rops.layernorm(h, *b["n1"], self.eps)
             qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"]).view(N, T, 3, self.heads, D)
             q, k, v = (qkv[:, :, j].transpose(1, 2) for j in range(3))
             a = F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(N * T, hid).contiguous()
             a = ops.linear(a, b["wo"], bias=b["bo"])
-            h = (h.float() + b["l1"].float() * a.float()).to(self.dtype)
-            y = rops.layernorm(h, *b["n2"], self.eps)
+            y, h = norms.branch_norm(a, h, gate=b["l1"], pre_w=b["n2"][0], pre_b=b["n2"][1], layer_norm=True, eps=self.eps)
             u = ops.linear(y, b["w1"], bias=b["b1"])
             if self.swiglu:
                 half = u.shape[1] // 2
@@ -107,7 +106,8 @@ class Dinov2Backbone:
             else:
                 u = rops.activation(u, "gelu")
             u = ops.linear(u, b["w2"], bias=b["b2"])
-            h = (h.float() + b["l2"].float() * u.float()).to(self.dtype)
+            w, b1 = self.blocks[li + 1]["n1"] if li + 1 < len(self.blocks) else (None, None)
+            y, h = norms.branch_norm(u, h, gate=b["l2"], pre_w=w, pre_b=b1, layer_norm=True, eps=self.eps)
             emit(li + 1)
         return outs
 

@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import ops
-from ..ops import recurrent as rops
+from ..ops import recurrent as rops, rotary
 from .vlm import VisionLanguage, _sub
 
 
@@ -71,7 +71,40 @@ class Qwen2ImageProcessor:
         return torch.cat(rows), grids
 
 
-class Qwen2VisionTower:
+def grid_positions(grids, merge: int) -> torch.Tensor:
+    """int32 [2, rows]: row and column of every patch, rows listed in merge-window order (``merge`` 1: raster order)."""
+    out = []
+    for t_, gh, gw in grids:
+        hp = torch.arange(gh, dtype=torch.int32)[:, None].expand(gh, gw)
+        wp = torch.arange(gw, dtype=torch.int32)[None, :].expand(gh, gw)
+        both = torch.stack([hp, wp]).reshape(2, gh // merge, merge, gw // merge, merge).permute(0, 1, 3, 2, 4).reshape(2, gh * gw)
+        out.append(both.repeat(1, t_))
+    return torch.cat(out, dim=1)
+
+
+class _AxialHeads:
+    """q, k and v of a tower's fused projection as its attention reads them: fp32 [heads, rows, D], q and k turned by their patch's
+    row (first half of the frequencies) and column."""
+
+    def _axial(self, grids, order=None, merge: int | None = None):
+        """For these grids: the function of the projection [rows, 3 * heads * D], and the rotation of fp32 [rows, heads, D] alone.
+        ``order``: the tower's own order of merge windows."""
+        merge = self.merge if merge is None else merge
+        pos = grid_positions(grids, merge).to(self.device)
+        if order is not None:
+            pos = pos.view(2, -1, merge ** 2)[:, order].reshape(2, -1).contiguous()
+        half = self.dim // self.heads // 2
+        inv = torch.cat([self.inv_freq, self.inv_freq]).to(self.device)
+        axes = (torch.arange(half) >= half // 2).int().to(self.device)
+        # (projections in fp32 on a GPU take the plain statement: the kernel reads bf16)
+        plain = self.device.type == "cuda" and self.dtype != torch.bfloat16
+        turn = lambda z: ops.reference.rotate_axes(z, pos, inv, axes, 2 * half)    # noqa: E731
+        if plain:
+            return lambda qkv: ops.reference.axial_rope(qkv, pos, inv, axes, self.heads, 2 * half), turn
+        return lambda qkv: rotary.axial_rope(qkv, pos, inv, axes, heads=self.heads, D=2 * half), turn
+
+
+class Qwen2VisionTower(_AxialHeads):
     """Patch embedding → blocks (LayerNorm, attention with 2-D rotary positions restricted to the
     image, quick-GELU MLP) → merger (LayerNorm, fold merge^2 rows, two linears with GELU)."""
 
@@ -102,38 +135,21 @@ class Qwen2VisionTower:
         D = self.dim // self.heads
         self.inv_freq = 1.0 / (10000.0 ** (torch.arange(0, D // 2, 2, dtype=torch.float32) / (D // 2)))
 
-    def _rot_angles(self, grids) -> torch.Tensor:
-        """[rows, D/2] rotary angles: the first D/4 frequencies turn with the patch's row, the rest with
-        its column, rows listed in merge-window order."""
-        m, out = self.merge, []
-        for t_, gh, gw in grids:
-            hp = torch.arange(gh)[:, None].expand(gh, gw).reshape(gh // m, m, gw // m, m).permute(0, 2, 1, 3).flatten()
-            wp = torch.arange(gw)[None, :].expand(gh, gw).reshape(gh // m, m, gw // m, m).permute(0, 2, 1, 3).flatten()
-            ang = torch.cat([hp[:, None].float() * self.inv_freq[None], wp[:, None].float() * self.inv_freq[None]], dim=1)
-            out.append(ang.repeat(t_, 1))
-        return torch.cat(out)
-
     @torch.no_grad()
     def forward(self, rows: torch.Tensor, grids) -> torch.Tensor:
         """``rows`` [R, C*tp*p*p] → [R / merge^2, text_hidden]."""
         from ..models.vision import _act
         x = ops.linear(F.pad(rows.to(self.device, self.dtype), (0, self.k_pad)).contiguous(), self.patch_w)
         R, H, D = x.shape[0], self.heads, self.dim // self.heads
-        ang = self._rot_angles(grids).to(self.device)
-        cos = torch.cat([ang.cos(), ang.cos()], dim=1)[:, None, :]       # [R, 1, D]
-        sin = torch.cat([ang.sin(), ang.sin()], dim=1)[:, None, :]
+        heads, _ = self._axial(grids)
         sizes = [t_ * gh * gw for t_, gh, gw in grids]
 
-        def rot(v):            # [R, H, D] float32
-            half = D // 2
-            return v * cos + torch.cat([-v[..., half:], v[..., :half]], dim=-1) * sin
         for b in self.blocks:
             y = rops.layernorm(x, b["n1w"], b["n1b"], 1e-6)
-            qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"]).view(R, 3, H, D)
-            q, k, v = rot(qkv[:, 0].float()), rot(qkv[:, 1].float()), qkv[:, 2].float()
+            q, k, v = heads(ops.linear(y, b["wqkv"], bias=b["bqkv"]))
             outs, o0 = [], 0
             for n in sizes:                                    # attention never crosses images
-                qi, ki, vi = (z[o0:o0 + n].transpose(0, 1)[None] for z in (q, k, v))
+                qi, ki, vi = (z[None, :, o0:o0 + n] for z in (q, k, v))
                 outs.append(F.scaled_dot_product_attention(qi, ki, vi)[0].transpose(0, 1).reshape(n, H * D))
                 o0 += n
             a = torch.cat(outs).to(self.dtype).contiguous()
@@ -145,7 +161,7 @@ class Qwen2VisionTower:
         return ops.linear(y, *self.m2)
 
 
-class Qwen25VisionTower:
+class Qwen25VisionTower(_AxialHeads):
     """Qwen2.5-VL tower: the Qwen2-VL layout with RMSNorm, a SwiGLU MLP and *windowed* attention. The
     merged-token groups (merge x merge patches) of an image are reordered window by window
     (``window_size`` pixels per side); most blocks attend inside a window, the blocks listed in
@@ -182,7 +198,6 @@ class Qwen25VisionTower:
         D = self.dim // self.heads
         self.inv_freq = 1.0 / (10000.0 ** (torch.arange(0, D // 2, 2, dtype=torch.float32) / (D // 2)))
 
-    _rot_angles = Qwen2VisionTower._rot_angles
 
     def _windows(self, grids):
         """Order of the merged-token groups (window by window) and the group count of every window."""
@@ -209,22 +224,16 @@ class Qwen25VisionTower:
         order, win_groups = self._windows(grids)
         order = order.to(self.device)
         x = x.view(R // unit, unit, self.dim)[order].reshape(R, self.dim).contiguous()
-        ang = self._rot_angles(grids).to(self.device).view(R // unit, unit, -1)[order].reshape(R, -1)
-        cos = torch.cat([ang.cos(), ang.cos()], dim=1)[:, None, :]
-        sin = torch.cat([ang.sin(), ang.sin()], dim=1)[:, None, :]
+        heads, _ = self._axial(grids, order)
         full_sizes = [gh * gw for t_, gh, gw in grids for _ in range(t_)]
         win_sizes = [g * unit for g in win_groups]
 
-        def rot(v):
-            half = D // 2
-            return v * cos + torch.cat([-v[..., half:], v[..., :half]], dim=-1) * sin
         for li, b in enumerate(self.blocks):
             y = ops.rmsnorm(x, b["n1"], 1e-6, 0.0)
-            qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"]).view(R, 3, H, D)
-            q, k, v = rot(qkv[:, 0].float()), rot(qkv[:, 1].float()), qkv[:, 2].float()
+            q, k, v = heads(ops.linear(y, b["wqkv"], bias=b["bqkv"]))
             outs, o0 = [], 0
             for n in (full_sizes if li in self.full_blocks else win_sizes):
-                qi, ki, vi = (z[o0:o0 + n].transpose(0, 1)[None] for z in (q, k, v))
+                qi, ki, vi = (z[None, :, o0:o0 + n] for z in (q, k, v))
                 outs.append(F.scaled_dot_product_attention(qi, ki, vi)[0].transpose(0, 1).reshape(n, H * D))
                 o0 += n
             a = torch.cat(outs).to(self.dtype).contiguous()
@@ -312,22 +321,16 @@ class Qwen3VisionTower(Qwen2VisionTower):
         x = ops.linear(F.pad(rows.to(self.device, self.dtype), (0, self.k_pad)).contiguous(), self.patch_w, bias=self.patch_b)
         x = (x.float() + self._pos_embed(grids).to(self.device)).to(self.dtype)
         R, H, D = x.shape[0], self.heads, self.dim // self.heads
-        ang = self._rot_angles(grids).to(self.device)
-        cos = torch.cat([ang.cos(), ang.cos()], dim=1)[:, None, :]
-        sin = torch.cat([ang.sin(), ang.sin()], dim=1)[:, None, :]
+        heads, _ = self._axial(grids)
         sizes = [gh * gw for t_, gh, gw in grids for _ in range(t_)]          # attention stays inside a frame
 
-        def rot(v):
-            half = D // 2
-            return v * cos + torch.cat([-v[..., half:], v[..., :half]], dim=-1) * sin
         deep = []
         for li, b in enumerate(self.blocks):
             y = rops.layernorm(x, b["n1w"], b["n1b"], 1e-6)
-            qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"]).view(R, 3, H, D)
-            q, k, v = rot(qkv[:, 0].float()), rot(qkv[:, 1].float()), qkv[:, 2].float()
+            q, k, v = heads(ops.linear(y, b["wqkv"], bias=b["bqkv"]))
             outs, o0 = [], 0
             for n in sizes:
-                qi, ki, vi = (z[o0:o0 + n].transpose(0, 1)[None] for z in (q, k, v))
+                qi, ki, vi = (z[None, :, o0:o0 + n] for z in (q, k, v))
                 outs.append(F.scaled_dot_product_attention(qi, ki, vi)[0].transpose(0, 1).reshape(n, H * D))
                 o0 += n
             a = torch.cat(outs).to(self.dtype).contiguous()
@@ -414,25 +417,21 @@ class Glm4vVisionTower(Qwen2VisionTower):
         if self.pos_table is not None:
             x = (x.float() + self._pos_embed(grids).to(self.device)).to(self.dtype)
         R, H, D = x.shape[0], self.heads, self.dim // self.heads
-        ang = self._rot_angles(grids).to(self.device)
-        cos = torch.cat([ang.cos(), ang.cos()], dim=1)[:, None, :]
-        sin = torch.cat([ang.sin(), ang.sin()], dim=1)[:, None, :]
+        heads, turn = self._axial(grids)
         sizes = [gh * gw for t_, gh, gw in grids for _ in range(t_)]
 
-        def rot(v):
-            half = D // 2
-            return v * cos + torch.cat([-v[..., half:], v[..., :half]], dim=-1) * sin
         for b in self.blocks:
             y = ops.rmsnorm(x, b["n1"], self.eps)
-            qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"]).view(R, 3, H, D)
-            q, k, v = qkv[:, 0].float(), qkv[:, 1].float(), qkv[:, 2].float()
-            if b["qn"] is not None:
+            qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"])
+            if b["qn"] is None:
+                q, k, v = heads(qkv)
+            else:
                 hn = lambda z, w: z * torch.rsqrt(z.pow(2).mean(-1, keepdim=True) + self.eps) * w.float()  # noqa: E731
-                q, k = hn(q, b["qn"]), hn(k, b["kn"])
-            q, k = rot(q), rot(k)
+                q, k, v = qkv.view(R, 3, H, D).float().unbind(1)
+                q, k, v = (z.transpose(0, 1) for z in (turn(hn(q, b["qn"])), turn(hn(k, b["kn"])), v))
             outs, o0 = [], 0
             for n in sizes:
-                qi, ki, vi = (z[o0:o0 + n].transpose(0, 1)[None] for z in (q, k, v))
+                qi, ki, vi = (z[None, :, o0:o0 + n] for z in (q, k, v))
                 outs.append(F.scaled_dot_product_attention(qi, ki, vi)[0].transpose(0, 1).reshape(n, H * D))
                 o0 += n
             x = ops.linear(torch.cat(outs).to(self.dtype).contiguous(), b["wo"], bias=b["bo"], residual=x)
@@ -511,30 +510,21 @@ class PaddleOcrVisionTower(Qwen2VisionTower):
         from ..models.vision import _act
         x = ops.linear(F.pad(rows.to(self.device, self.dtype), (0, self.k_pad)).contiguous(), self.patch_w, bias=self.patch_b)
         tab = self.pos_table.float().view(1, self.side, self.side, -1).permute(0, 3, 1, 2)
-        pos, ang = [], []
+        pos = []
         for t_, gh, gw in grids:
             pe = F.interpolate(tab, size=(gh, gw), mode="bilinear", align_corners=False)
             pos.append(pe.permute(0, 2, 3, 1).reshape(gh * gw, -1).repeat(t_, 1))
-            hp = torch.arange(gh)[:, None].expand(gh, gw).flatten().float()
-            wp = torch.arange(gw)[None, :].expand(gh, gw).flatten().float()
-            ang.append(torch.cat([hp[:, None] * self.inv_freq[None], wp[:, None] * self.inv_freq[None]], dim=1).repeat(t_, 1))
         x = (x.float() + torch.cat(pos).to(self.device)).to(self.dtype)
-        ang = torch.cat(ang).to(self.device)
-        cos = torch.cat([ang.cos(), ang.cos()], dim=1)[:, None, :]
-        sin = torch.cat([ang.sin(), ang.sin()], dim=1)[:, None, :]
+        heads, _ = self._axial(grids, merge=1)            # (rows in raster order)
         R, H, D = x.shape[0], self.heads, self.dim // self.heads
         sizes = [gh * gw for t_, gh, gw in grids for _ in range(t_)]
 
-        def rot(v):
-            half = D // 2
-            return v * cos + torch.cat([-v[..., half:], v[..., :half]], dim=-1) * sin
         for b in self.blocks:
             y = rops.layernorm(x, *b["n1"], self.eps)
-            qkv = ops.linear(y, b["wqkv"], bias=b["bqkv"]).view(R, 3, H, D)
-            q, k, v = rot(qkv[:, 0].float()), rot(qkv[:, 1].float()), qkv[:, 2].float()
+            q, k, v = heads(ops.linear(y, b["wqkv"], bias=b["bqkv"]))
             outs, o0 = [], 0
             for n in sizes:
-                qi, ki, vi = (z[o0:o0 + n].transpose(0, 1)[None] for z in (q, k, v))
+                qi, ki, vi = (z[None, :, o0:o0 + n] for z in (q, k, v))
                 outs.append(F.scaled_dot_product_attention(qi, ki, vi)[0].transpose(0, 1).reshape(n, H * D))
                 o0 += n
             x = ops.linear(torch.cat(outs).to(self.dtype).contiguous(), b["wo"], bias=b["bo"], residual=x)
