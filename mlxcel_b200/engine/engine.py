@@ -28,7 +28,7 @@ from ..config import ModelConfig
 from ..host_runtime import BlockManager, TickAction, TickState, decide_tick, prefill_piece
 from ..models.decoder import DecoderModel, StepBatch
 from .params import FinishReason, SamplingParams, SeqStatus
-from .sampler import Sampler
+from .sampler import Sampler, TokenLogprob
 
 
 @dataclass
@@ -1114,7 +1114,7 @@ class Engine:
                 return FinishReason.STOP
         s.output.append(tok)
         if lp is not None and p.logprobs:
-            s.logprobs.append(float(lp))
+            s.logprobs.append(lp if isinstance(lp, TokenLogprob) else float(lp))
         if len(s.output) >= p.max_tokens:
             return FinishReason.LENGTH
         if not self._ctx_shift:

@@ -15,6 +15,13 @@ import math
 import torch
 
 from .. import ops
+from ..ops import logprobs
+
+
+class TokenLogprob(float):
+    """The log probability of a drawn token; ``top`` lists the most likely tokens at its place as (id, log probability)."""
+
+    top: list = []
 
 
 class Sampler:
@@ -97,7 +104,21 @@ class Sampler:
         for i, s in enumerate(seqs):
             if not s.params.fused_eligible:
                 toks[i], lps[i] = self._extended(work[i], s)
+        asked = [i for i, s in enumerate(seqs) if s.params.logprobs and s.params.top_logprobs > 0]
+        if asked:
+            self._alternatives(work, seqs, asked, toks, lps)
         return toks, lps
+
+    @staticmethod
+    def _alternatives(work, seqs, rows, toks, lps) -> None:
+        """Replaces the log probabilities of rows that ask for alternatives by ones that carry them (of the distribution the token was
+        drawn from, before the filters; at most ``logprobs.MAX_TOP``)."""
+        k = min(max(seqs[i].params.top_logprobs for i in rows), logprobs.MAX_TOP, work.shape[1])
+        ids = torch.tensor([toks[i] for i in rows], dtype=torch.int32).to(work.device)
+        r = logprobs.token_logprobs(work if len(rows) == work.shape[0] else work[rows], ids, k)
+        for i, lp, at, top in zip(rows, r.logprob.tolist(), r.top_ids.tolist(), r.top_logprobs.tolist()):
+            lps[i] = TokenLogprob(lp)
+            lps[i].top = [(t, v) for t, v in zip(at, top) if v > float("-inf")][:seqs[i].params.top_logprobs]     # (masked ones are none)
 
     # ------------------------------------------------------------------ extended chain
     def _extended(self, l: torch.Tensor, s) -> tuple[int, float]:

@@ -2,8 +2,8 @@
 
 Reference: ``DirectEngine::loglikelihoods`` (src/lib/mlxcel-core/src/engine/direct.rs) and the
 perplexity example (examples/perplexity.rs). One prefill forward over a private KV pool per window;
-the logits are taken for every row, in slices, so that a long window never holds ``[T, vocab]`` fp32
-at once. State-space and hybrid executors get a scratch state slot that is released afterwards.
+the logits of a slice of rows are reduced as they are made (or row slices of them are held), so that a long
+window never holds ``[T, vocab]`` fp32 at once. State-space and hybrid executors get a scratch state slot that is released afterwards.
 """
 from __future__ import annotations
 
@@ -12,6 +12,7 @@ import math
 import torch
 
 from ..models.decoder import StepBatch
+from ..ops.logprobs import TokenLogprobs, token_logprobs
 
 _SCRATCH_SEQ = -7
 
@@ -43,20 +44,30 @@ def prefill_hidden(model, cfg, ids: list[int], block_size: int = 16) -> torch.Te
 
 
 @torch.inference_mode()
-def sequence_logprobs(model, cfg, ids: list[int], block_size: int = 16, row_chunk: int = 512) -> torch.Tensor:
-    """``log p(ids[t] | ids[:t])`` for t = 1 .. T-1 as an fp32 CPU tensor [T-1]."""
+def sequence_scores(model, cfg, ids: list[int], block_size: int = 16, row_chunk: int = 512, top: int = 0) -> TokenLogprobs:
+    """For t = 1 .. T-1, on the CPU: ``log p(ids[t] | ids[:t])``, the entropy of that distribution and the ``top`` most likely tokens
+    with their log probabilities."""
     T = len(ids)
     if T < 2:
-        return torch.zeros(0)
+        none = torch.zeros(0)
+        return TokenLogprobs(none, none, none, torch.zeros(0, top, dtype=torch.int32), torch.zeros(0, top))
     dev = model.device
     h = prefill_hidden(model, cfg, ids, block_size)
     tgt = torch.tensor(ids[1:], dtype=torch.long, device=dev)
-    out = []
+    own = getattr(model, "token_logprobs", None)
+    if own is not None and not top:
+        row_chunk = max(row_chunk, 8192)                     # (no logits are held for these rows, or few)
+    parts = []
     for r0 in range(0, T - 1, row_chunk):
         rows = torch.arange(r0, min(r0 + row_chunk, T - 1), device=dev)
-        lp = torch.log_softmax(model.logits(h, rows).float(), dim=-1)
-        out.append(lp.gather(1, tgt[rows, None])[:, 0].cpu())
-    return torch.cat(out)
+        want = tgt[r0:r0 + row_chunk]
+        parts.append(own(h, rows, want, top) if own is not None else token_logprobs(model.logits(h, rows), want, top))
+    return TokenLogprobs(*(torch.cat(p).cpu() for p in zip(*parts)))
+
+
+def sequence_logprobs(model, cfg, ids: list[int], block_size: int = 16, row_chunk: int = 512) -> torch.Tensor:
+    """``log p(ids[t] | ids[:t])`` for t = 1 .. T-1 as an fp32 CPU tensor [T-1]."""
+    return sequence_scores(model, cfg, ids, block_size, row_chunk).logprob
 
 
 def perplexity(model, cfg, ids: list[int], window: int = 2048, stride: int | None = None, block_size: int = 16,

@@ -21,7 +21,7 @@ import torch
 
 from .. import ops
 from ..config import ModelConfig
-from ..ops import KVLayer
+from ..ops import KVLayer, logprobs as lops, norms, rotary
 from ..ops.reference import rope_inv_freq
 from .weights import LayerWeights, ModelWeights, QuantizedTensor
 
@@ -143,6 +143,7 @@ class DecoderModel:
             self.inv_freq_local = rope_inv_freq(cfg.rot_dim, cfg.extra["rope_local_theta"], None)[0].to(dev)
         self.device = dev
         self._ssq = None
+        self._mrope_axes = None            # the axis each rotary frequency turns with (multimodal positions)
         self.fold_attn = self.fold_mlp = False
         self.nope_layers = frozenset(cfg.extra.get("nope_layers", ()))
         self.layernorm = cfg.extra.get("norm") == "layernorm"
@@ -257,16 +258,16 @@ class DecoderModel:
             q_norm = k_norm = None
             rot_dim = 0
         if b.positions3 is not None and rot_dim and cfg.extra.get("mrope_section"):
-            # rows with three different rotary positions: rotate here (each frequency takes the position
-            # of its section), the kernel only appends
-            from ..ops import reference as ref
-            T0, nqk = qkv.shape[0], self.Hq + self.Hkv
-            x3 = qkv.view(T0, self.Hq + 2 * self.Hkv, self.D)
-            rot = ref.apply_mrope(x3[:, :nqk], b.positions3, self.inv_freq, cfg.extra["mrope_section"], self.mscale,
-                                  interleaved=bool(cfg.extra.get("mrope_interleaved")), rot_dim=rot_dim,
-                                  traditional=cfg.rope_traditional)
-            qkv = torch.cat([rot.to(qkv.dtype), x3[:, nqk:]], dim=1).reshape(T0, -1).contiguous()
-            rot_dim = 0
+            # rows with three different rotary positions: each frequency takes the position of its section
+            win = window > 0 and b.slot_mapping_win is not None
+            if self._mrope_axes is None:
+                self._mrope_axes = rotary.section_axes(cfg.extra["mrope_section"], rot_dim // 2,
+                                                       bool(cfg.extra.get("mrope_interleaved"))).to(qkv.device)
+            rotary.mrope_append(qkv, b.positions3, b.slot_mapping_win if win else b.slot_mapping, self.inv_freq, self._mrope_axes, kv,
+                                Hq=self.Hq, Hkv=self.Hkv, D=self.D, rot_dim=rot_dim, traditional=cfg.rope_traditional,
+                                mscale=self.mscale, q_norm_w=q_norm, k_norm_w=k_norm, norm_eps=cfg.rms_norm_eps,
+                                out=qkv[:, : self.Hq * self.D])
+            return self._attend(qkv, b, kv, window, lw.sinks, win)
         use_win = window > 0 and b.slot_mapping_win is not None     # this layer's KV lives in the window pool
         ops.rope_append(qkv, b.positions, b.slot_mapping_win if use_win else b.slot_mapping,
                         self.inv_freq_local if local else self.inv_freq, kv,
@@ -484,47 +485,45 @@ class DecoderModel:
             for li, lw in enumerate(w.layers):
                 a = self._attention(li, lw, h, b, kv_layers[li])
                 o = self.comm.row_parallel_linear(a, lw.wo, lw.bo, None)
-                h = (h.float() + ops.rmsnorm(o, lw.post_attn_norm, eps, wb).float()).to(h.dtype)
+                _, h = norms.branch_norm(o, h, post_w=lw.post_attn_norm, eps=eps, w_bias=wb)
                 if cfg.is_moe:
                     raise NotImplementedError("post-norm-only MoE blocks")
                 o = self.comm.row_parallel_linear(self._mlp(lw, h), lw.w_down, lw.b_down, None)
-                h = (h.float() + ops.rmsnorm(o, lw.post_mlp_norm, eps, wb).float()).to(h.dtype)
+                _, h = norms.branch_norm(o, h, post_w=lw.post_mlp_norm, eps=eps, w_bias=wb)
             return h
+        # Branches with a norm behind them or a scale end in one kernel: that norm, the scale, the sum, and the norm in front of the
+        # next sub-layer (``x``; None where it is still to be taken)
+        joined = cfg.post_norms or res_mult != 1.0
+        x = None
         for li, lw in enumerate(w.layers):
             kv = kv_layers[li]
-            x = ops.rmsnorm(h, lw.ln1, eps, wb)
+            if x is None:
+                x = ops.rmsnorm(h, lw.ln1, eps, wb)
             a = self._attention(li, lw, x, b, kv)
             if lw.attn_gate is not None:                    # AFMoE: sigmoid gate from the layer input
                 a = (a.float() * torch.sigmoid(_linear_any(x, lw.attn_gate).float())).to(a.dtype)
-            if cfg.post_norms or res_mult != 1.0:
+            if joined:
                 o = self.comm.row_parallel_linear(a, lw.wo, lw.bo, None)
-                if cfg.post_norms:
-                    o = ops.rmsnorm(o, lw.post_attn_norm, eps, wb)
-                if res_mult != 1.0:
-                    o = (o.float() * res_mult).to(o.dtype)
-                x, h = ops.add_rmsnorm(o, h, lw.ln2, eps, wb)
+                x, h = norms.branch_norm(o, h, post_w=lw.post_attn_norm if cfg.post_norms else None, scale=res_mult, pre_w=lw.ln2,
+                                         eps=eps, w_bias=wb)
             else:
                 h = self.comm.row_parallel_linear(a, lw.wo, lw.bo, h)
                 x = ops.rmsnorm(h, lw.ln2, eps, wb)
-            if cfg.is_moe and lw.router_w is not None and res_mult != 1.0:              # GraniteMoE: scaled expert branch
-                o = self._moe(lw, x, torch.zeros_like(h))
-                h = (h.float() + o.float() * res_mult).to(h.dtype)
-            elif cfg.is_moe and lw.router_w is not None and cfg.post_norms:     # AFMoE: a norm after the MoE block
-                o = ops.rmsnorm(self._moe(lw, x, torch.zeros_like(h)), lw.post_mlp_norm, eps, wb)
-                h = (h.float() + o.float()).to(h.dtype)
-            elif cfg.is_moe and lw.router_w is not None:
-                h = self._moe(lw, x, h)
-            else:
-                m = self._mlp(lw, x)
-                if cfg.post_norms or res_mult != 1.0:
-                    o = self.comm.row_parallel_linear(m, lw.w_down, lw.b_down, None)
-                    if cfg.post_norms:
-                        o = ops.rmsnorm(o, lw.post_mlp_norm, eps, wb)
-                    if res_mult != 1.0:
-                        o = (o.float() * res_mult).to(o.dtype)
-                    h = (h.float() + o.float()).to(h.dtype) if not h.is_cuda else h.add_(o)
+            moe = cfg.is_moe and lw.router_w is not None
+            if joined:
+                if moe:                                     # (AFMoE: a norm after the MoE block; GraniteMoE: a scaled one)
+                    o = self._moe(lw, x, torch.zeros_like(h))
                 else:
-                    h = self.comm.row_parallel_linear(m, lw.w_down, lw.b_down, h)
+                    o = self.comm.row_parallel_linear(self._mlp(lw, x), lw.w_down, lw.b_down, None)
+                nxt = w.layers[li + 1].ln1 if li + 1 < len(w.layers) and b.deepstack is None else None
+                x, h = norms.branch_norm(o, h, post_w=lw.post_mlp_norm if cfg.post_norms else None, scale=res_mult, pre_w=nxt, eps=eps,
+                                         w_bias=wb)
+            else:
+                if moe:
+                    h = self._moe(lw, x, h)
+                else:
+                    h = self.comm.row_parallel_linear(self._mlp(lw, x), lw.w_down, lw.b_down, h)
+                x = None
             h = self._deepstack(li, h, b)
             self._capture(li, h)
         return h
@@ -620,6 +619,18 @@ class DecoderModel:
             c = cfg.final_logit_softcap
             lg = (torch.tanh(lg.float() / c) * c).to(lg.dtype)
         return lg
+
+    def token_logprobs(self, h: torch.Tensor, rows: torch.Tensor | None, ids: torch.Tensor, top: int = 0):
+        """:class:`~mlxcel_b200.ops.logprobs.TokenLogprobs` of tokens ``ids`` behind the selected rows. Without alternatives, on one GPU
+        and with dense head weights the logits stay on the chip (and are not rounded)."""
+        cfg, w = self.cfg, self.w
+        if top or self.comm.tp_size != 1 or isinstance(w.lm_head, QuantizedTensor) or type(self).logits is not DecoderModel.logits:
+            return lops.token_logprobs(self.logits(h, rows), ids, top)
+        if rows is not None:
+            h = h.index_select(0, rows)
+        x = self._norm(h, w.final_norm, w.extra.get("final_norm_b"))
+        return lops.head_logprobs(x, w.lm_head, ids, bias=w.extra.get("lm_head_b"), scale=1.0 / float(cfg.extra.get("logits_scaling", 1.0)),
+                                  softcap=float(cfg.final_logit_softcap))
 
     def forward(self, b: StepBatch, kv_layers: list[KVLayer]) -> torch.Tensor:
         h = self.forward_hidden(b, kv_layers)

@@ -427,6 +427,17 @@ def create_app(state: ServerState) -> FastAPI:
         return {"input_tokens": len(tk.encode(state.render(msgs)))}
 
     # ------------------------------------------------------------------ completions
+    def _ranked(pairs) -> dict:
+        """{token text: log probability} of (id, log probability) pairs, most likely first."""
+        out: dict = {}
+        for t, lp in pairs:
+            out.setdefault(tk.decode([t]), lp)
+        return out
+
+    def _alternatives(lp) -> dict:
+        top = getattr(lp, "top", None)
+        return {"top_logprobs": [{"token": tk.decode([t]), "logprob": v} for t, v in top]} if top else {}
+
     async def _run_text(prompt_ids, sp, constraint=None, public_id=None):
         text, lps, toks, final = [], [], [], None
         async for ev in _generate(state, prompt_ids, sp, constraint, public_id=public_id):
@@ -499,10 +510,15 @@ def create_app(state: ServerState) -> FastAPI:
         if body.get("echo"):
             # prompt scoring (what evaluation harnesses ask for): the prompt comes back with the log-probability
             # of each of its tokens given the ones before; ``max_tokens: 0`` scores without generating
-            from ..engine.scoring import sequence_logprobs
+            from ..engine.scoring import sequence_scores
+            from ..ops.logprobs import MAX_TOP
             eng = state.worker.engine
-            plp = await asyncio.get_running_loop().run_in_executor(
-                None, lambda: sequence_logprobs(eng.model, eng.cfg, ids, eng.ecfg.block_size).tolist())
+            # alternatives at every place of the prompt: ``top_logprobs``, or the count that ``logprobs`` gives
+            many = int(body.get("logprobs") or 0) if not isinstance(body.get("logprobs"), bool) else 0
+            many = min(max(0, sp.top_logprobs or many), MAX_TOP, eng.cfg.vocab_size)
+            scores = await asyncio.get_running_loop().run_in_executor(
+                None, lambda: sequence_scores(eng.model, eng.cfg, ids, eng.ecfg.block_size, top=many))
+            plp = scores.logprob.tolist()
             ptoks = [tk.decode([t], skip_special_tokens=False) for t in ids]
             offs, pos = [], 0
             for piece in ptoks:
@@ -520,6 +536,9 @@ def create_app(state: ServerState) -> FastAPI:
                       "logprobs": {"tokens": ptoks + [tk.decode([t]) for t in gen_toks],
                                    "token_logprobs": [None] + plp + (gen_lps if sp.logprobs else [None] * len(gen_toks)),
                                    "text_offset": offs}}
+            if many:
+                choice["logprobs"]["top_logprobs"] = ([None] + [_ranked(zip(i, v)) for i, v in zip(scores.top_ids.tolist(), scores.top_logprobs.tolist())]
+                                                      + [_ranked(getattr(lp, "top", [])) for lp in gen_lps if sp.logprobs])
             return {"id": cid, "object": "text_completion", "created": created, "model": state.model_id, "choices": [choice],
                     "usage": usage or {"prompt_tokens": len(ids), "completion_tokens": 0, "total_tokens": len(ids)}}
         try:
@@ -532,6 +551,8 @@ def create_app(state: ServerState) -> FastAPI:
             choice = {"index": i, "text": text, "finish_reason": _finish_openai(fin.finish_reason, False)}
             if sp.logprobs:
                 choice["logprobs"] = {"token_logprobs": lps, "tokens": [tk.decode([t]) for t in toks]}
+                if sp.top_logprobs > 0:
+                    choice["logprobs"]["top_logprobs"] = [_ranked(getattr(lp, "top", [])) for lp in lps]
             choices.append(choice)
         return {"id": cid, "object": "text_completion", "created": created, "model": state.model_id,
                 "choices": choices, "usage": _sum_usage(runs), "timings": runs[0][3].timings}
@@ -699,7 +720,7 @@ def create_app(state: ServerState) -> FastAPI:
                 msg["tool_calls"] = [c.to_openai() for c in calls]
             choice = {"index": i, "message": msg, "finish_reason": _finish_openai(fin.finish_reason, bool(calls))}
             if sp.logprobs:
-                choice["logprobs"] = {"content": [{"token": tk.decode([t]), "logprob": lp} for t, lp in zip(toks, lps)]}
+                choice["logprobs"] = {"content": [{"token": tk.decode([t]), "logprob": lp, **_alternatives(lp)} for t, lp in zip(toks, lps)]}
             choices.append(choice)
         return {"id": cid, "object": "chat.completion", "created": created, "model": state.model_id,
                 "choices": choices, "usage": _sum_usage(runs), "timings": runs[0][3].timings}
