@@ -176,9 +176,24 @@ int mx_add_rmsnorm(const void* x, const void* residual, const void* weight, void
 // The step between two sub-layers (bf16, or fp32 where `fp32`; strides in elements):
 // h = residual + scale * gate * rms(x) * (post_w + w_bias), y = norm(h) * (pre_w + w_bias) + pre_b. NULL operands are left out (without
 // pre_w there is no y); layer_norm: the second norm is a layer norm. h may be x or residual itself.
-int mx_branch_norm(const void* x, long long ldx, const void* residual, long long ldr, const void* post_w, const void* gate,
-                   const void* pre_w, const void* pre_b, void* h, long long ldh, void* y, long long ldy, int rows, int dim,
-                   float scale, float eps, float w_bias, int layer_norm, int fp32, void* stream);
+typedef struct MxBranchNorm {
+  const void* x;
+  long long ldx;
+  const void* residual;
+  long long ldr;
+  const void* post_w;
+  const void* gate;
+  const void* pre_w;
+  const void* pre_b;
+  void* h;
+  long long ldh;
+  void* y;
+  long long ldy;
+  int rows, dim;
+  float scale, eps, w_bias;
+  int layer_norm, fp32;
+} MxBranchNorm;
+int mx_branch_norm(const MxBranchNorm* args, void* stream);
 
 // Per-head RMSNorm over the last dimension of [tokens, heads, head_dim] (Qwen3 q/k norm), in place.
 int mx_head_rmsnorm(void* x, const void* weight, int tokens, int heads, int head_dim,
@@ -205,10 +220,27 @@ int mx_rope_append(void* qkv, const int* positions, const int* slot_mapping, con
 // [T, (Hq + 2 Hkv) * D] bf16 with row stride ldqkv; rotated q goes to q_out (row stride ldq; q's own columns are fine), k and v into the
 // pool (layouts of mx_rope_append) at `slots`, those outside [0, n_slots) nowhere. pairs: columns (2i, 2i + 1) turn together, else
 // (i, i + rot_dim / 2). q_norm_w / k_norm_w: per-head rms norm before the rotation. mscale multiplies the rotated columns.
-int mx_mrope_append(const void* qkv, long long ldqkv, void* q_out, long long ldq, const int* positions, long long ldp, int axes,
-                    const int* axis, const int* slots, long long n_slots, const float* inv_freq, void* k_pool, void* v_pool,
-                    void* k_meta, void* v_meta, const void* q_norm_w, const void* k_norm_w, float norm_eps, int T, int Hq,
-                    int Hkv, int D, int rot_dim, int block_size, int pairs, float mscale, int kv_bits, void* stream);
+typedef struct MxMropeAppend {
+  const void* qkv;
+  long long ldqkv;
+  void* q_out;
+  long long ldq;
+  const int* positions;
+  long long ldp;
+  const int* axis;
+  const int* slots;
+  long long n_slots;
+  const float* inv_freq;
+  void* k_pool;
+  void* v_pool;
+  void* k_meta;
+  void* v_meta;
+  const void* q_norm_w;
+  const void* k_norm_w;
+  int axes, T, Hq, Hkv, D, rot_dim, block_size, pairs, kv_bits;
+  float norm_eps, mscale;
+} MxMropeAppend;
+int mx_mrope_append(const MxMropeAppend* args, void* stream);
 // q, k (rotated, pairs (i, i + D / 2)) and v of qkv [R, 3 * H * D] bf16 as fp32 [H, R, D].
 int mx_axial_rope(const void* qkv, long long ldqkv, float* q, float* k, float* v, const int* positions, long long ldp, int axes,
                   const int* axis, const float* inv_freq, int R, int H, int D, void* stream);
@@ -276,9 +308,20 @@ long long mx_sample_scratch_floats(int B, int V);
 // Of every row of logits [R, V] (bf16 or fp32, row stride ld; the distribution is that of softcap * tanh((x + bias) * scale / softcap),
 // softcap 0: none): log probabilities of n_ids tokens ids[R, n_ids] (NaN outside the vocabulary), entropy, log normaliser, the `top`
 // most likely tokens (ties: lowest index) with their log probabilities. NaN logits count as -inf.
-int mx_token_logprobs(const void* logits, int fp32, long long ld, const void* ids, int ids64, int n_ids, const void* bias,
-                      int bias_fp32, float scale, float softcap, float* logprob, float* entropy, float* lse, int* top_ids,
-                      float* top_logprobs, int top, int R, int V, void* stream);
+typedef struct MxTokenLogprobs {
+  const void* logits;
+  long long ld;
+  const void* ids;
+  const void* bias;
+  float* logprob;
+  float* entropy;
+  float* lse;
+  int* top_ids;
+  float* top_logprobs;
+  int fp32, ids64, n_ids, bias_fp32, top, R, V;
+  float scale, softcap;
+} MxTokenLogprobs;
+int mx_token_logprobs(const MxTokenLogprobs* args, void* stream);
 // The same without alternatives for the logits x[M, K] @ w[V, K]^T (bf16, fp32 sums), which are not stored. partials: fp32
 // [3 * ceil(V / 256) + 1, M]; status: the device status word of bounded waits. -10: strides or addresses that TMA does not take.
 int mx_head_logprobs(const void* x, const void* w, const void* ids, int ids64, const void* bias, int bias_fp32, float scale,

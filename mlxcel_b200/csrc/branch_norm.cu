@@ -218,17 +218,16 @@ static int launch_branch_norm(const BranchNormParams& p, int rows, cudaStream_t 
 
 }  // namespace mx
 
-extern "C" int mx_branch_norm(const void* x, long long ldx, const void* residual, long long ldr, const void* post_w, const void* gate,
-                              const void* pre_w, const void* pre_b, void* h, long long ldh, void* y, long long ldy, int rows, int dim,
-                              float scale, float eps, float w_bias, int layer_norm, int fp32, void* stream_) {
+extern "C" int mx_branch_norm(const MxBranchNorm* a, void* stream_) {
   using namespace mx;
-  if (rows <= 0) return 0;
-  if (dim <= 0 || dim > 32768 || x == nullptr || h == nullptr || (pre_w != nullptr && y == nullptr)) return -1;
-  const BranchNormParams p{x, residual, post_w, gate, pre_w, pre_b, h, y, ldx, ldr, ldh, ldy, dim, scale, eps, w_bias};
+  if (a->rows <= 0) return 0;
+  if (a->dim <= 0 || a->dim > 32768 || a->x == nullptr || a->h == nullptr || (a->pre_w != nullptr && a->y == nullptr)) return -1;
+  const BranchNormParams p{a->x, a->residual, a->post_w, a->gate, a->pre_w, a->pre_b, a->h, a->y, a->ldx, a->ldr, a->ldh, a->ldy, a->dim, a->scale, a->eps, a->w_bias};
+  const int rows = a->rows, dim = a->dim, fp32 = a->fp32, layer_norm = a->layer_norm;
   const int v = fp32 ? 4 : 8;
-  bool wide = dim % v == 0 && ldx % v == 0 && ldr % v == 0 && ldh % v == 0 && ldy % v == 0;
-  for (const void* a : {x, residual, post_w, gate, pre_w, pre_b, static_cast<const void*>(h), static_cast<const void*>(y)})
-    wide = wide && aligned_to(a, 16);
+  bool wide = dim % v == 0 && a->ldx % v == 0 && a->ldr % v == 0 && a->ldh % v == 0 && a->ldy % v == 0;
+  for (const void* t : {a->x, a->residual, a->post_w, a->gate, a->pre_w, a->pre_b, static_cast<const void*>(a->h), static_cast<const void*>(a->y)})
+    wide = wide && aligned_to(t, 16);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (fp32) {
     if (wide) return layer_norm ? launch_branch_norm<float, 4, true>(p, rows, stream) : launch_branch_norm<float, 4, false>(p, rows, stream);

@@ -411,16 +411,17 @@ static cudaError_t launch_token_logprobs(const LpParams& p, int rows, cudaStream
 
 }  // namespace mx
 
-extern "C" int mx_token_logprobs(const void* logits, int fp32, long long ld, const void* ids, int ids64, int n_ids, const void* bias,
-                                 int bias_fp32, float scale, float softcap, float* logprob, float* entropy, float* lse, int* top_ids,
-                                 float* top_logprobs, int top, int R, int V, void* stream_) {
+extern "C" int mx_token_logprobs(const MxTokenLogprobs* a, void* stream_) {
   using namespace mx;
-  if (R <= 0) return 0;
-  if (V <= 0 || V > (1 << 30) || R > (1 << 27) || top < 0 || top > V || top > kLpTop || n_ids < 0 || scale <= 0.f || softcap < 0.f) return -1;
-  const LpParams p{logits, ids, bias, logprob, entropy, lse, top_ids, top_logprobs, ld, V, n_ids, ids64, bias_fp32, top, scale, softcap};
+  if (a->R <= 0) return 0;
+  if (a->V <= 0 || a->V > (1 << 30) || a->R > (1 << 27) || a->top < 0 || a->top > a->V || a->top > kLpTop || a->n_ids < 0 || !(a->scale > 0.f) ||
+      !(a->softcap >= 0.f))
+    return -1;
+  const LpParams p{a->logits, a->ids, a->bias, a->logprob, a->entropy, a->lse, a->top_ids, a->top_logprobs, a->ld, a->V, a->n_ids, a->ids64, a->bias_fp32,
+                   a->top, a->scale, a->softcap};
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   cudaError_t e;
-  if (fp32) e = top ? launch_token_logprobs<float, true>(p, R, stream) : launch_token_logprobs<float, false>(p, R, stream);
-  else e = top ? launch_token_logprobs<__nv_bfloat16, true>(p, R, stream) : launch_token_logprobs<__nv_bfloat16, false>(p, R, stream);
+  if (a->fp32) e = a->top ? launch_token_logprobs<float, true>(p, a->R, stream) : launch_token_logprobs<float, false>(p, a->R, stream);
+  else e = a->top ? launch_token_logprobs<__nv_bfloat16, true>(p, a->R, stream) : launch_token_logprobs<__nv_bfloat16, false>(p, a->R, stream);
   return static_cast<int>(e);
 }

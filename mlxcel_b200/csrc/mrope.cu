@@ -386,33 +386,31 @@ static int mrope_width(int D, int rot, uintptr_t addresses, long long strides) {
 
 }  // namespace mx
 
-extern "C" int mx_mrope_append(const void* qkv, long long ldqkv, void* q_out, long long ldq, const int* positions, long long ldp, int axes,
-                               const int* axis, const int* slots, long long n_slots, const float* inv_freq, void* k_pool, void* v_pool,
-                               void* k_meta, void* v_meta, const void* q_norm_w, const void* k_norm_w, float norm_eps, int T, int Hq,
-                               int Hkv, int D, int rot_dim, int block_size, int pairs, float mscale, int kv_bits, void* stream_) {
+extern "C" int mx_mrope_append(const MxMropeAppend* a, void* stream_) {
   using namespace mx;
+  const int T = a->T, D = a->D, rot_dim = a->rot_dim, kv_bits = a->kv_bits;
   if (T <= 0) return 0;
-  if (D <= 0 || D > kMropeMaxDim || rot_dim < 0 || rot_dim > D || rot_dim % 2 || Hq < 0 || Hkv < 0 || axes < 1 || block_size < 1) return -1;
-  if ((kv_bits != 16 && kv_bits != 8 && kv_bits != 4) || (kv_bits != 16 && (D % 64 || k_meta == nullptr || v_meta == nullptr))) return -1;
+  if (D <= 0 || D > kMropeMaxDim || rot_dim < 0 || rot_dim > D || rot_dim % 2 || a->Hq < 0 || a->Hkv < 0 || a->axes < 1 || a->block_size < 1) return -1;
+  if ((kv_bits != 16 && kv_bits != 8 && kv_bits != 4) || (kv_bits != 16 && (D % 64 || a->k_meta == nullptr || a->v_meta == nullptr))) return -1;
   MropeParams p{};
-  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
-  p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.slots = slots;
-  p.k_pool = k_pool, p.v_pool = v_pool;
-  p.k_meta = static_cast<__nv_bfloat16*>(k_meta), p.v_meta = static_cast<__nv_bfloat16*>(v_meta);
-  p.q_norm_w = static_cast<const __nv_bfloat16*>(q_norm_w), p.k_norm_w = static_cast<const __nv_bfloat16*>(k_norm_w);
-  p.ang = {positions, axis, inv_freq, ldp, axes, rot_dim / 2};
-  p.ldqkv = ldqkv, p.ldq = ldq, p.n_slots = n_slots;
-  p.Hq = Hq, p.Hkv = Hkv, p.D = D, p.block_size = block_size, p.pairs = pairs;
-  p.eps = norm_eps, p.mscale = mscale;
+  p.qkv = static_cast<const __nv_bfloat16*>(a->qkv);
+  p.q_out = static_cast<__nv_bfloat16*>(a->q_out);
+  p.slots = a->slots;
+  p.k_pool = a->k_pool, p.v_pool = a->v_pool;
+  p.k_meta = static_cast<__nv_bfloat16*>(a->k_meta), p.v_meta = static_cast<__nv_bfloat16*>(a->v_meta);
+  p.q_norm_w = static_cast<const __nv_bfloat16*>(a->q_norm_w), p.k_norm_w = static_cast<const __nv_bfloat16*>(a->k_norm_w);
+  p.ang = {a->positions, a->axis, a->inv_freq, a->ldp, a->axes, rot_dim / 2};
+  p.ldqkv = a->ldqkv, p.ldq = a->ldq, p.n_slots = a->n_slots;
+  p.Hq = a->Hq, p.Hkv = a->Hkv, p.D = D, p.block_size = a->block_size, p.pairs = a->pairs;
+  p.eps = a->norm_eps, p.mscale = a->mscale;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   cudaError_t e;
   auto bits_of = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
-  const int w = kv_bits == 16 ? mrope_width(D, rot_dim, bits_of(qkv) | bits_of(q_out) | bits_of(k_pool) | bits_of(v_pool) | bits_of(q_norm_w) | bits_of(k_norm_w),
-                                            ldqkv | ldq) : 0;
+  const int w = kv_bits == 16 ? mrope_width(D, rot_dim, bits_of(a->qkv) | bits_of(a->q_out) | bits_of(a->k_pool) | bits_of(a->v_pool) | bits_of(a->q_norm_w) |
+                                            bits_of(a->k_norm_w), a->ldqkv | a->ldq) : 0;
   if (w != 0) {
     const int lanes = D / (2 * w), per = mrope_tokens(T), blocks = (T + per - 1) / per;
-    const bool norm = q_norm_w != nullptr || k_norm_w != nullptr;
+    const bool norm = a->q_norm_w != nullptr || a->k_norm_w != nullptr;
 #define MX_MROPE(W_, L_)                                                                                                          \
     e = norm ? launch_kernel(mrope_append_vec_kernel<W_, L_, true>, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)      \
              : launch_kernel(mrope_append_vec_kernel<W_, L_, false>, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)

@@ -93,13 +93,12 @@ def _declare(lib) -> None:
         "mx_qstream_ahead": [_i, _i, _ll, _i],
         "mx_qstream": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp],
         "mx_row_ssq": [_vp, _i, _i, _ll, _vp, _vp],
-        "mx_branch_norm": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _ll, _i, _i, _f, _f, _f, _i, _i, _vp],
-        "mx_mrope_append": [_vp, _ll, _vp, _ll, _vp, _ll, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i,
-                            _i, _f, _i, _vp],
+        "mx_branch_norm": [ctypes.c_char_p, _vp],
+        "mx_mrope_append": [ctypes.c_char_p, _vp],
         "mx_axial_rope": [_vp, _ll, _vp, _vp, _vp, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _vp],
         "mx_pages": [_i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp],
         "mx_head_logprobs": [_vp, _vp, _vp, _i, _vp, _i, _f, _f, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
-        "mx_token_logprobs": [_vp, _i, _ll, _vp, _i, _i, _vp, _i, _f, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
+        "mx_token_logprobs": [ctypes.c_char_p, _vp],
         "mx_add_rmsnorm": [_vp, _vp, _vp, _vp, _vp, _i, _i, _f, _f, _vp],
         "mx_head_rmsnorm": [_vp, _vp, _i, _i, _i, _ll, _f, _vp],
         "mx_rope_append": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i,
@@ -210,13 +209,19 @@ def stream() -> int:
 def launch_on(device: torch.device, name: str, *args) -> None:
     """Calls entry ``name`` on the current stream of ``device`` (appended as the last argument), whichever device is current."""
     fn = getattr(load(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    idx = device.index
+    if idx is None or idx == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(torch.cuda.current_device() if idx is None else idx))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _raw_stream(idx))
     count_launch()
-    check(rc, name)
+    if rc:
+        check(rc, name)
+
+
+# (the stream's handle without a Stream object around it, where torch has the call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
 
 # ----------------------------------------------------------------------------- workspaces

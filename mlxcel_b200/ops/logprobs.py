@@ -2,6 +2,7 @@
 (``csrc/logprobs.cu``) or straight from hidden rows and the head's weights."""
 from __future__ import annotations
 
+import struct
 from typing import NamedTuple
 
 import torch
@@ -9,6 +10,7 @@ import torch
 from . import _lib, linear, reference as ref
 
 MAX_TOP = 64
+_ARGS = struct.Struct("PqPPPPPPPiiiiiiiff")        # MxTokenLogprobs of csrc/api.h
 FUSED_ROWS = 256        # above, head_logprobs keeps its logits on the chip
 
 
@@ -49,14 +51,15 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, bia
     if logits.stride(1) != 1 and V > 1 or R > 1 and logits.stride(0) < V:
         raise ValueError("the logits of a row have to be adjacent and rows apart")
     ids = ids.contiguous()
-    f = dict(dtype=torch.float32, device=logits.device)
-    r = TokenLogprobs(torch.empty(ids.shape, **f), torch.empty(R, **f), torch.empty(R, **f),
-                      torch.empty(R, top, dtype=torch.int32, device=logits.device), torch.empty(R, top, **f))
+    # one buffer for all results (they are a few words per row)
+    n, k = ids.numel(), R * top
+    logprob, entropy, lse, best, at = torch.empty(n + 2 * R + 2 * k, dtype=torch.float32, device=logits.device).split([n, R, R, k, k])
+    r = TokenLogprobs(logprob if ids.dim() == 1 else logprob.view(ids.shape), entropy, lse, at.view(torch.int32).view(R, top), best.view(R, top))
     if R:
-        _lib.launch_on(logits.device, "mx_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
-                       int(ids.dtype == torch.int64), ids.numel() // R, _lib.ptr(bias), int(bias is not None and bias.dtype == torch.float32),
-                       float(scale), float(softcap), r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), r.top_ids.data_ptr(),
-                       r.top_logprobs.data_ptr(), top, R, V)
+        _lib.launch_on(logits.device, "mx_token_logprobs", _ARGS.pack(
+            logits.data_ptr(), logits.stride(0), ids.data_ptr(), 0 if bias is None else bias.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
+            lse.data_ptr(), at.data_ptr(), best.data_ptr(), logits.dtype == torch.float32, ids.dtype == torch.int64, n // R,
+            bias is not None and bias.dtype == torch.float32, top, R, V, scale, softcap))
     return r
 
 

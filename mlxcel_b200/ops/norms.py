@@ -3,9 +3,14 @@ the residual and the norm in front of the next sub-layer (``csrc/branch_norm.cu`
 sub-layer, with scaled branches or with per-channel branch scales take it at every layer."""
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib, reference as ref
+
+_ARGS = struct.Struct("PqPqPPPPPqPqiifffii")        # MxBranchNorm of csrc/api.h
+_TYPES = (torch.bfloat16, torch.float32)
 
 
 def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w: torch.Tensor | None = None,
@@ -21,29 +26,36 @@ def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w
     goes (``x`` or ``residual`` itself is fine)."""
     if x.dim() != 2:
         raise ValueError(f"branch_norm takes rows [rows, dim], not {tuple(x.shape)}")
-    rows, dim = x.shape
-    if x.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"branch_norm takes bf16 or fp32 rows, not {x.dtype}")
+    rows, dim = shape = x.shape
+    dtype, dev = x.dtype, x.get_device()
+    if dtype not in _TYPES:
+        raise ValueError(f"branch_norm takes bf16 or fp32 rows, not {dtype}")
     for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
-            raise ValueError(f"{name} has to be like x: {tuple(x.shape)} {x.dtype} on {x.device}")
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != dev):
+            raise ValueError(f"{name} has to be like x: {tuple(shape)} {dtype} on {x.device}")
     for name, t in (("post_w", post_w), ("gate", gate), ("pre_w", pre_w), ("pre_b", pre_b)):
-        if t is not None and (t.shape != (dim,) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous()):
-            raise ValueError(f"{name} has to be a contiguous [{dim}] {x.dtype} tensor on {x.device}")
+        if t is not None and (t.dtype != dtype or t.dim() != 1 or t.numel() != dim or t.get_device() != dev or not t.is_contiguous()):
+            raise ValueError(f"{name} has to be a contiguous [{dim}] {dtype} tensor on {x.device}")
     if pre_b is not None and (pre_w is None or not layer_norm):
         raise ValueError("pre_b belongs to a layer norm (pre_w, layer_norm=True)")
-    if dim < 1 or dim > 32768:
+    if not 1 <= dim <= 32768:
         raise ValueError(f"rows of 1 to 32768 elements are covered, not {dim}")
     if not x.is_cuda:
         y, h = ref.branch_norm(x, residual, post_w, gate, scale, pre_w, pre_b, layer_norm, eps, w_bias)
         return y, h if out is None else out.copy_(h)
+    strides = []
     for name, t in (("x", x), ("residual", residual), ("out", out)):
-        if t is not None and (t.stride(1) != 1 and dim > 1 or rows > 1 and t.stride(0) < dim):
-            raise ValueError(f"the elements of a row of {name} have to be adjacent and its rows apart")
-    h = torch.empty(rows, dim, dtype=x.dtype, device=x.device) if out is None else out
-    y = torch.empty(rows, dim, dtype=x.dtype, device=x.device) if pre_w is not None else None
+        ld = dim
+        if t is not None:
+            ld, one = t.stride()
+            if one != 1 and dim > 1 or rows > 1 and ld < dim:
+                raise ValueError(f"the elements of a row of {name} have to be adjacent and its rows apart")
+        strides.append(ld)
+    h = torch.empty(shape, dtype=dtype, device=x.device) if out is None else out
+    y = torch.empty(shape, dtype=dtype, device=x.device) if pre_w is not None else None
     if rows:
-        _lib.launch_on(x.device, "mx_branch_norm", x.data_ptr(), x.stride(0), _lib.ptr(residual), 0 if residual is None else residual.stride(0),
-                       _lib.ptr(post_w), _lib.ptr(gate), _lib.ptr(pre_w), _lib.ptr(pre_b), h.data_ptr(), h.stride(0), _lib.ptr(y), dim, rows, dim,
-                       float(scale), float(eps), float(w_bias), int(layer_norm), int(x.dtype == torch.float32))
+        at = lambda t: 0 if t is None else t.data_ptr()    # noqa: E731
+        _lib.launch_on(x.device, "mx_branch_norm", _ARGS.pack(
+            x.data_ptr(), strides[0], at(residual), strides[1], at(post_w), at(gate), at(pre_w), at(pre_b), h.data_ptr(), strides[2], at(y), dim,
+            rows, dim, scale, eps, w_bias, layer_norm, dtype == torch.float32))
     return y, h

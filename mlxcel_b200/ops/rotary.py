@@ -5,9 +5,13 @@ Frequency ``i`` of the rotated half turns with the position of axis ``axes[i]``;
 sections."""
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import KVLayer, _lib, reference as ref
+
+_ARGS = struct.Struct("PqPqPqPPqPPPPPPPiiiiiiiiiff")        # MxMropeAppend of csrc/api.h
 
 
 def section_axes(sections, half: int, interleaved: bool = False) -> torch.Tensor:
@@ -77,10 +81,12 @@ def mrope_append(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch
         raise ValueError(f"a {bits}-bit pool of {kv.k.dtype} is not covered")
     q = torch.empty(T, Hq * D, dtype=qkv.dtype, device=qkv.device) if out is None else out
     if T:
-        _lib.launch_on(qkv.device, "mx_mrope_append", qkv.data_ptr(), qkv.stride(0), q.data_ptr(), q.stride(0), positions.data_ptr(),
-                       positions.stride(0), positions.shape[0], axes.data_ptr(), slot_mapping.data_ptr(), kv.k.shape[0] * kv.block_size,
-                       inv_freq.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), _lib.ptr(kv.k_meta), _lib.ptr(kv.v_meta), _lib.ptr(q_norm_w),
-                       _lib.ptr(k_norm_w), float(norm_eps), T, Hq, Hkv, D, rot_dim, kv.block_size, int(traditional), float(mscale), bits)
+        at = lambda t: 0 if t is None else t.data_ptr()    # noqa: E731
+        _lib.launch_on(qkv.device, "mx_mrope_append", _ARGS.pack(
+            qkv.data_ptr(), qkv.stride(0), q.data_ptr(), q.stride(0), positions.data_ptr(), positions.stride(0), axes.data_ptr(),
+            slot_mapping.data_ptr(), kv.k.shape[0] * kv.block_size, inv_freq.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), at(kv.k_meta),
+            at(kv.v_meta), at(q_norm_w), at(k_norm_w), positions.shape[0], T, Hq, Hkv, D, rot_dim, kv.block_size, traditional, bits, norm_eps,
+            mscale))
     return q
 
 
