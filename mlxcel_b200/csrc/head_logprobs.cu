@@ -6,7 +6,9 @@
 // token's logit where the tile holds it. A second launch joins the column tiles of each row.
 // Logits of 2047 rows over 128256 tokens would be 1 GB of fp32; what is written instead is 12 MB. The logits are never rounded.
 //
-// Bound by the tensor cores: a tile's products take 8 K cycles an SM, its epilogue about 3400 beside them.
+// Bound by the tensor cores under the power cap: a tile's products take 8 K cycles an SM, its epilogue about 3000 beside them, whose
+// instructions cost power and with it clock. Measured, in a row (us): 2047 rows, K 4096, V 128256 1770 (1.21 PFLOP/s; 1910 with the
+// changes of SHAPED made in any case); the same product by gemm_pair.cu, which writes 525 MB of bf16 logits, 1750, by cuBLAS 1550.
 #include <cooperative_groups.h>
 
 #include "api.h"
@@ -34,6 +36,8 @@ __device__ __forceinline__ long long head_id(const HeadParams& p, int m) {
   return p.ids64 ? static_cast<const long long*>(p.ids)[m] : static_cast<const int*>(p.ids)[m];
 }
 
+// SHAPED: the products are not the logits yet (a bias, a scale or a soft cap).
+template <bool SHAPED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGpThreads, 1)
 head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
   extern __shared__ uint8_t hl_smem[];
@@ -161,9 +165,16 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         float z[32], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          z[i] = c + i < valid ? lp_transform(__uint_as_float(r[i]), f0 + c + i, p.bias, p.bias_fp32, p.scale, p.softcap) : -INFINITY;
-          top = fmaxf(top, z[i]);
+          z[i] = __uint_as_float(r[i]);
+          if constexpr (SHAPED) z[i] = lp_transform(z[i], min(f0 + c + i, p.V - 1), p.bias, p.bias_fp32, p.scale, p.softcap);
         }
+        if (c + 32 > valid) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i >= valid) z[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, z[i]);            // (NaN is dropped here and by the floor below: it counts as -inf)
         if (top > a.m) a = lp_rescale(a, top);
         if (lp_plain(a.m)) {
           const float low = lp_floor(a.m);
@@ -182,7 +193,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         if (own_col >= c && own_col < c + 32) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (own_col == c + i) own = z[i];
+            if (own_col == c + i) own = z[i] != z[i] ? -INFINITY : z[i];
         }
       }
       tc_fence_before_sync();
@@ -245,13 +256,15 @@ extern "C" int mx_head_logprobs(const void* x, const void* w, const void* ids, i
                scale, softcap};
   CUtensorMap map_x, map_w;
   if (!make_tensor_map_bf16(&map_x, x, M, K, ldx, 128, kGpBK) || !make_tensor_map_bf16(&map_w, w, V, K, ldw, 128, kGpBK)) return -4;
-  static bool allowed[64] = {};
-  cudaError_t e = allow_shared(head_logprobs_kernel, kGpSmem, allowed);
+  const bool shaped = bias != nullptr || scale != 1.f || softcap > 0.f;
+  auto kern = shaped ? head_logprobs_kernel<true> : head_logprobs_kernel<false>;
+  static bool allowed[2][64] = {};
+  cudaError_t e = allow_shared(kern, kGpSmem, allowed[shaped]);
   if (e != cudaSuccess) return static_cast<int>(e);
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n, most = device_sm_count() / 2;
   if (tiles > 0x7fffffffll) return -1;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  e = launch_kernel(head_logprobs_kernel, dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most)), dim3(kGpThreads), kGpSmem, stream, map_x, map_w, p);
+  e = launch_kernel(kern, dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most)), dim3(kGpThreads), kGpSmem, stream, map_x, map_w, p);
   if (e != cudaSuccess) return static_cast<int>(e);
   return static_cast<int>(launch_kernel(head_join_kernel, dim3((M + 31) / 32), dim3(1024), 0, stream, p));
 }
