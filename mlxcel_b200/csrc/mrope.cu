@@ -182,9 +182,9 @@ __device__ __forceinline__ bool unit_columns(int u, int half, int pairs, int& c0
   }
   return turns;
 }
-// Turns a lane's 2 W values by the W angles from cs, sn on.
+// Turns a lane's 2 W values by the W angles from cs, sn on (which carry the scale).
 template <int W>
-__device__ __forceinline__ void turn_unit(float (&a)[W], float (&b)[W], const float* cs, const float* sn, int pairs, float mscale) {
+__device__ __forceinline__ void turn_unit(float (&a)[W], float (&b)[W], const float* cs, const float* sn, int pairs) {
   float c[W], s[W];
 #pragma unroll
   for (int i = 0; i < W; i += 4) {
@@ -195,60 +195,79 @@ __device__ __forceinline__ void turn_unit(float (&a)[W], float (&b)[W], const fl
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) {
       const float x0 = a[2 * i], y0 = a[2 * i + 1], x1 = b[2 * i], y1 = b[2 * i + 1];
-      a[2 * i] = (x0 * c[i] - y0 * s[i]) * mscale;
-      a[2 * i + 1] = (y0 * c[i] + x0 * s[i]) * mscale;
-      b[2 * i] = (x1 * c[W / 2 + i] - y1 * s[W / 2 + i]) * mscale;
-      b[2 * i + 1] = (y1 * c[W / 2 + i] + x1 * s[W / 2 + i]) * mscale;
+      a[2 * i] = x0 * c[i] - y0 * s[i];
+      a[2 * i + 1] = y0 * c[i] + x0 * s[i];
+      b[2 * i] = x1 * c[W / 2 + i] - y1 * s[W / 2 + i];
+      b[2 * i + 1] = y1 * c[W / 2 + i] + x1 * s[W / 2 + i];
     }
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const float x = a[i], y = b[i];
-      a[i] = (x * c[i] - y * s[i]) * mscale;
-      b[i] = (y * c[i] + x * s[i]) * mscale;
+      a[i] = x * c[i] - y * s[i];
+      b[i] = y * c[i] + x * s[i];
     }
   }
 }
 
+// (token, head) of an index that grows by a fixed step, without a division per step.
+struct HeadWalk {
+  int t, s;
+  __device__ __forceinline__ HeadWalk(int item, int heads) : t(item / heads), s(item % heads) {}
+  __device__ __forceinline__ void step(int by, int heads) {
+    s += by;
+    while (s >= heads) s -= heads, ++t;
+  }
+};
+
 template <int W, int LPH, bool NORM>
-__global__ void __launch_bounds__(kMropeThreads, 4) mrope_append_vec_kernel(const MropeParams p, int tokens, int per_block) {
+__global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_vec_kernel(const MropeParams p, int tokens, int per_block) {
   using Vec = typename MropeVec<W>::type;
   __shared__ __align__(16) float cs[kMropeTokens * kMropeMaxDim / 2], sn[kMropeTokens * kMropeMaxDim / 2];
-  constexpr int HPI = kMropeThreads / LPH;
+  __shared__ long long kept[kMropeTokens];                      // where a token's first head goes in the pool; below 0: nowhere
+  constexpr int HPI = kMropeThreads / LPH, HPW = 32 / LPH;      // heads at once: of the CTA, of a warp
   pdl_trigger();
   pdl_wait();
   const int t0 = blockIdx.x * per_block, rows = min(per_block, tokens - t0), heads = p.Hq + 2 * p.Hkv, half = p.ang.half, D = p.D;
-  const int g = threadIdx.x / LPH, u = threadIdx.x % LPH, items = rows * heads;
+  const int g = threadIdx.x / LPH, u = threadIdx.x % LPH;
   int c0, c1;
   const bool turns = unit_columns<W>(u, half, p.pairs, c0, c1), live = u * 2 * W < D;
+  const __nv_bfloat16* src = p.qkv + t0 * p.ldqkv;
+  const long long page_head = static_cast<long long>(p.block_size) * D;
   Vec v[2][2];
-  auto load = [&](int item, Vec (&x)[2]) {
-    if (live && item < items) {
-      const int t = item / heads;
-      const __nv_bfloat16* src = p.qkv + (t0 + t) * p.ldqkv + static_cast<long long>(item - t * heads) * D;
-      x[0] = *reinterpret_cast<const Vec*>(src + c0);
-      x[1] = *reinterpret_cast<const Vec*>(src + c1);
+  HeadWalk ahead(g, heads);
+  auto load = [&](Vec (&x)[2]) {
+    if (live && ahead.t < rows) {
+      const __nv_bfloat16* from = src + ahead.t * p.ldqkv + ahead.s * D;
+      x[0] = *reinterpret_cast<const Vec*>(from + c0);
+      x[1] = *reinterpret_cast<const Vec*>(from + c1);
     }
+    ahead.step(HPI, heads);
   };
-  load(g, v[0]);
-  load(g + HPI, v[1]);
+  load(v[0]);
+  load(v[1]);
+  if (threadIdx.x < rows) {
+    const long long slot = p.slots[t0 + threadIdx.x], blk = slot / p.block_size;
+    kept[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : (blk * p.Hkv * p.block_size + (slot - blk * p.block_size)) * D;
+  }
   for (int i = threadIdx.x; i < rows * half; i += kMropeThreads) {
     const int t = i / half;
-    axis_angle(p.ang, t0 + t, i - t * half, sn[i], cs[i]);
+    float sine, cosine;
+    axis_angle(p.ang, t0 + t, i - t * half, sine, cosine);
+    sn[i] = sine * p.mscale;
+    cs[i] = cosine * p.mscale;
   }
   __syncthreads();
-  // whole warps stay in the loop: the norm's sums are exchanged between lanes
-  for (int first = g - g % (32 / LPH > 0 ? 32 / LPH : 1), item = g, k = 0; first < items; first += HPI, item += HPI, k ^= 1) {
+  HeadWalk at(g, heads);
+  auto work = [&](Vec (&x)[2]) {
     float a[W], b[W];
-    const bool here = live && item < items;
-    const int t = item / heads, s = item - t * heads;
-    const bool is_q = s < p.Hq, is_v = s >= p.Hq + p.Hkv;
+    const bool here = live && at.t < rows;
+    const bool is_q = at.s < p.Hq, is_v = at.s >= p.Hq + p.Hkv;
     if (here) {
-      MropeVec<W>::widen(k ? v[1][0] : v[0][0], a);
-      MropeVec<W>::widen(k ? v[1][1] : v[0][1], b);
+      MropeVec<W>::widen(x[0], a);
+      MropeVec<W>::widen(x[1], b);
     }
-    if (k) load(item + 2 * HPI, v[1]);
-    else load(item + 2 * HPI, v[0]);
+    load(x);
     if constexpr (NORM) {
       float ss = 0.f;
       if (here) {
@@ -269,20 +288,26 @@ __global__ void __launch_bounds__(kMropeThreads, 4) mrope_append_vec_kernel(cons
         for (int i = 0; i < W; ++i) b[i] *= rstd * w[i];
       }
     }
-    if (!here) continue;
-    if (turns && !is_v) turn_unit<W>(a, b, cs + t * half + W * u, sn + t * half + W * u, p.pairs, p.mscale);
-    __nv_bfloat16* dst;
-    if (is_q) {
-      dst = p.q_out + (t0 + t) * p.ldq + static_cast<long long>(s) * D;
-    } else {
-      const long long slot = p.slots[t0 + t];
-      if (slot < 0 || slot >= p.n_slots) continue;              // a row without a slot leaves the pool alone
-      const long long blk = slot / p.block_size;
-      const int head = s - p.Hq - (is_v ? p.Hkv : 0);
-      dst = static_cast<__nv_bfloat16*>(is_v ? p.v_pool : p.k_pool) + ((blk * p.Hkv + head) * p.block_size + (slot - blk * p.block_size)) * D;
+    if (here) {
+      if (turns && !is_v) turn_unit<W>(a, b, cs + at.t * half + W * u, sn + at.t * half + W * u, p.pairs);
+      __nv_bfloat16* dst = nullptr;
+      if (is_q) {
+        dst = p.q_out + (t0 + at.t) * p.ldq + at.s * D;
+      } else if (kept[at.t] >= 0) {                             // (a row without a slot leaves the pool alone)
+        const int head = at.s - p.Hq - (is_v ? p.Hkv : 0);
+        dst = static_cast<__nv_bfloat16*>(is_v ? p.v_pool : p.k_pool) + kept[at.t] + head * page_head;
+      }
+      if (dst != nullptr) {
+        *reinterpret_cast<Vec*>(dst + c0) = MropeVec<W>::narrow(a);
+        *reinterpret_cast<Vec*>(dst + c1) = MropeVec<W>::narrow(b);
+      }
     }
-    *reinterpret_cast<Vec*>(dst + c0) = MropeVec<W>::narrow(a);
-    *reinterpret_cast<Vec*>(dst + c1) = MropeVec<W>::narrow(b);
+    at.step(HPI, heads);
+  };
+  // whole warps stay in the loop (it goes by the warp's first head), as the norm's sums are exchanged between lanes
+  for (int left = rows * heads - (g - g % HPW); left > 0; left -= 2 * HPI) {
+    work(v[0]);
+    if (left > HPI) work(v[1]);
   }
 }
 
@@ -319,55 +344,59 @@ __global__ void __launch_bounds__(kMropeThreads) axial_rope_kernel(const AxialPa
   }
 }
 
-template <int W, int LPH>
-__global__ void __launch_bounds__(kMropeThreads, 4) axial_rope_vec_kernel(const AxialParams p, int per_block) {
+// Units of 2 W columns of all heads (q, k, v) of up to 4 rows follow one another over the threads.
+template <int W>
+__global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) axial_rope_vec_kernel(const AxialParams p, int per_block) {
   using Vec = typename MropeVec<W>::type;
   __shared__ __align__(16) float cs[kMropeTokens * kMropeMaxDim / 2], sn[kMropeTokens * kMropeMaxDim / 2];
-  constexpr int HPI = kMropeThreads / LPH;
   pdl_trigger();
   pdl_wait();
   const long long t0 = static_cast<long long>(blockIdx.x) * per_block;
-  const int rows = static_cast<int>(min(static_cast<long long>(per_block), p.rows - t0)), half = p.ang.half, D = p.D;
-  const int g = threadIdx.x / LPH, u = threadIdx.x % LPH, items = rows * 3 * p.H;
-  int c0, c1;
-  unit_columns<W>(u, half, 0, c0, c1);
-  const bool live = u * 2 * W < D;
-  // neighbouring groups take neighbouring rows of one head: their results are adjacent
-  auto place = [&](int item, int& t, int& h) {
-    h = item / rows;                                            // q of all heads, k, v
-    t = item - h * rows;
+  const int rows = static_cast<int>(min(static_cast<long long>(per_block), p.rows - t0)), half = p.ang.half, D = p.D, heads = 3 * p.H;
+  const int units = D / (2 * W), u_step = kMropeThreads % units, h_step = kMropeThreads / units;
+  struct Place {
+    int u;
+    HeadWalk at;
   };
+  auto step = [&](Place& x) {
+    x.u += u_step;
+    const int carry = x.u >= units;
+    if (carry) x.u -= units;
+    x.at.step(h_step + carry, heads);
+  };
+  const __nv_bfloat16* src = p.qkv + t0 * p.ldqkv;
+  Place ahead{static_cast<int>(threadIdx.x) % units, HeadWalk(threadIdx.x / units, heads)}, now = ahead;
   Vec v[2][2];
-  auto load = [&](int item, Vec (&x)[2]) {
-    if (live && item < items) {
-      int t, h;
-      place(item, t, h);
-      const __nv_bfloat16* src = p.qkv + (t0 + t) * p.ldqkv + static_cast<long long>(h) * D;
-      x[0] = *reinterpret_cast<const Vec*>(src + c0);
-      x[1] = *reinterpret_cast<const Vec*>(src + c1);
+  auto load = [&](Vec (&x)[2]) {
+    if (ahead.at.t < rows) {
+      const __nv_bfloat16* from = src + ahead.at.t * p.ldqkv + ahead.at.s * D + ahead.u * W;
+      x[0] = *reinterpret_cast<const Vec*>(from);
+      x[1] = *reinterpret_cast<const Vec*>(from + half);
     }
+    step(ahead);
   };
-  load(g, v[0]);
-  load(g + HPI, v[1]);
+  load(v[0]);
+  load(v[1]);
   for (int i = threadIdx.x; i < rows * half; i += kMropeThreads) axis_angle(p.ang, t0 + i / half, i % half, sn[i], cs[i]);
   __syncthreads();
-  if (!live) return;
-  for (int item = g, k = 0; item < items; item += HPI, k ^= 1) {
+  auto work = [&](Vec (&x)[2]) {
     float a[W], b[W];
-    MropeVec<W>::widen(k ? v[1][0] : v[0][0], a);
-    MropeVec<W>::widen(k ? v[1][1] : v[0][1], b);
-    if (k) load(item + 2 * HPI, v[1]);
-    else load(item + 2 * HPI, v[0]);
-    int t, h;
-    place(item, t, h);
-    const int part = h / p.H;
-    if (part < 2) turn_unit<W>(a, b, cs + t * half + W * u, sn + t * half + W * u, 0, 1.f);
-    float* dst = (part == 0 ? p.q : part == 1 ? p.k : p.v) + (static_cast<long long>(h - part * p.H) * p.rows + t0 + t) * D;
+    MropeVec<W>::widen(x[0], a);
+    MropeVec<W>::widen(x[1], b);
+    load(x);
+    const int part = (now.at.s >= p.H) + (now.at.s >= 2 * p.H), h = now.at.s - part * p.H, angle = now.at.t * half + W * now.u;
+    if (part < 2) turn_unit<W>(a, b, cs + angle, sn + angle, 0);
+    float* dst = (part == 0 ? p.q : part == 1 ? p.k : p.v) + (h * p.rows + t0 + now.at.t) * D + W * now.u;
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      *reinterpret_cast<float4*>(dst + c0 + i) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
-      *reinterpret_cast<float4*>(dst + c1 + i) = make_float4(b[i], b[i + 1], b[i + 2], b[i + 3]);
+      *reinterpret_cast<float4*>(dst + i) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+      *reinterpret_cast<float4*>(dst + half + i) = make_float4(b[i], b[i + 1], b[i + 2], b[i + 3]);
     }
+    step(now);
+  };
+  while (now.at.t < rows) {
+    work(v[0]);
+    if (now.at.t < rows) work(v[1]);
   }
 }
 
@@ -377,9 +406,9 @@ static int mrope_tokens(int T) {
   while (n > 1 && T < 4 * n * device_sm_count()) n /= 2;
   return n;
 }
-// Columns per access (8, 4; 0: not in vectors) for heads of D whose first rot columns turn.
-static int mrope_width(int D, int rot, uintptr_t addresses, long long strides) {
-  for (int w : {8, 4})
+// Columns per access (`most` or 4; 0: not in vectors) for heads of D whose first rot columns turn.
+static int mrope_width(int most, int D, int rot, uintptr_t addresses, long long strides) {
+  for (int w = most; w >= 4; w -= 4)
     if (rot > 0 && D % (2 * w) == 0 && rot % (2 * w) == 0 && strides % w == 0 && addresses % (2 * w) == 0) return w;
   return 0;
 }
@@ -406,7 +435,9 @@ extern "C" int mx_mrope_append(const MxMropeAppend* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   cudaError_t e;
   auto bits_of = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
-  const int w = kv_bits == 16 ? mrope_width(D, rot_dim, bits_of(a->qkv) | bits_of(a->q_out) | bits_of(a->k_pool) | bits_of(a->v_pool) | bits_of(a->q_norm_w) |
+  // Accesses of 8 bytes leave room for more warps, those of 16 bytes take fewer instructions: 1031 tokens of 32 + 4 heads 8.1 us against 10.8,
+  // 8191 of 64 + 16 heads with norms 81 against 73.
+  const int w = kv_bits == 16 ? mrope_width(mrope_tokens(T) == kMropeTokens ? 8 : 4, D, rot_dim, bits_of(a->qkv) | bits_of(a->q_out) | bits_of(a->k_pool) | bits_of(a->v_pool) | bits_of(a->q_norm_w) |
                                             bits_of(a->k_norm_w), a->ldqkv | a->ldq) : 0;
   if (w != 0) {
     const int lanes = D / (2 * w), per = mrope_tokens(T), blocks = (T + per - 1) / per;
@@ -435,14 +466,12 @@ extern "C" int mx_axial_rope(const void* qkv, long long ldqkv, float* q, float* 
   if (R <= 0 || H <= 0) return 0;
   if (D <= 0 || D > kMropeMaxDim || D % 2 || axes < 1) return -1;
   AxialParams p{static_cast<const __nv_bfloat16*>(qkv), q, k, v, {positions, axis, inv_freq, ldp, axes, D / 2}, ldqkv, R, H, D};
-  const int w = mrope_width(D, D, reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v),
+  // (16-byte accesses: 33 us where 8-byte ones take 26, 5476 patches of 16 heads of 80)
+  const int w = mrope_width(4, D, D, reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v),
                             ldqkv);
   if (w != 0) {
-    const int lanes = D / (2 * w), per = mrope_tokens(R), blocks = (R + per - 1) / per;
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    auto run = [&](auto kern) { return static_cast<int>(launch_kernel(kern, dim3(blocks), dim3(kMropeThreads), 0, stream, p, per)); };
-    if (w == 8) return lanes <= 4 ? run(axial_rope_vec_kernel<8, 4>) : lanes <= 8 ? run(axial_rope_vec_kernel<8, 8>) : run(axial_rope_vec_kernel<8, 16>);
-    return lanes <= 8 ? run(axial_rope_vec_kernel<4, 8>) : lanes <= 16 ? run(axial_rope_vec_kernel<4, 16>) : run(axial_rope_vec_kernel<4, 32>);
+    const int per = mrope_tokens(R), blocks = (R + per - 1) / per;
+    return static_cast<int>(launch_kernel(axial_rope_vec_kernel<4>, dim3(blocks), dim3(kMropeThreads), 0, static_cast<cudaStream_t>(stream_), p, per));
   }
   return static_cast<int>(launch_kernel(axial_rope_kernel, dim3(R), dim3(kMropeThreads), 0, static_cast<cudaStream_t>(stream_), p));
 }

@@ -11,7 +11,10 @@ from . import _lib, linear, reference as ref
 
 MAX_TOP = 64
 _ARGS = struct.Struct("PqPPPPPPPiiiiiiiff")        # MxTokenLogprobs of csrc/api.h
-FUSED_ROWS = 256        # above, head_logprobs keeps its logits on the chip
+# head_logprobs keeps its logits on the chip, unless few rows meet large weights: there both forms read the weights at the pace of the
+# memory, and the smaller tiles of `linear` are the faster ones. us on the chip / through memory: 8 rows, 128256 x 4096 217 / 171, 64
+# rows 210 / 191, 100 rows 215 / 222, 256 rows 244 / 480; 8 rows, 50257 x 1024 49 / 61, 5000 x 512 27 / 59.
+FEW_ROWS, LARGE_WEIGHTS = 64, 1 << 28
 
 
 class TokenLogprobs(NamedTuple):
@@ -83,7 +86,7 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: 
     r = TokenLogprobs(torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, 0, dtype=torch.int32, device=x.device),
                       torch.empty(R, 0, **f))
     K = x.shape[1]
-    if R > FUSED_ROWS and x.dtype == torch.bfloat16 and not (K % 8 or x.stride(0) % 8 or w.stride(0) % 8 or (x.data_ptr() | w.data_ptr()) % 16):
+    if R and (R > FEW_ROWS or V * K <= LARGE_WEIGHTS) and x.dtype == torch.bfloat16 and not (K % 8 or x.stride(0) % 8 or w.stride(0) % 8 or (x.data_ptr() | w.data_ptr()) % 16):
         partials = torch.empty(3 * (-(-V // 256)) + 1, R, **f)
         ids = ids.contiguous()
         _lib.launch_on(x.device, "mx_head_logprobs", x.data_ptr(), w.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), _lib.ptr(bias),
@@ -92,7 +95,11 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: 
                        _lib.workspace(x.device).data_ptr())
         return r
     part = max(1, (1 << 26) // V)                 # rows whose logits are held at once: 256 MB
+    if R == 0:
+        return r
     with torch.cuda.device(x.device):
+        if R <= part:
+            return token_logprobs(linear(x, w, out_fp32=True, w_fresh=True), ids, bias=bias, scale=scale, softcap=softcap)
         for r0 in range(0, R, part):
             got = token_logprobs(linear(x[r0:r0 + part], w, out_fp32=True, w_fresh=True), ids[r0:r0 + part], bias=bias, scale=scale, softcap=softcap)
             for whole, piece in zip(r[:3], got[:3]):
