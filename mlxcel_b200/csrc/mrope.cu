@@ -224,6 +224,7 @@ template <int W, int LPH, bool NORM>
 __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_vec_kernel(const MropeParams p, int tokens, int per_block) {
   using Vec = typename MropeVec<W>::type;
   __shared__ __align__(16) float cs[kMropeTokens * kMropeMaxDim / 2], sn[kMropeTokens * kMropeMaxDim / 2];
+  __shared__ __align__(16) float norm_w[NORM ? 2 : 1][NORM ? kMropeMaxDim : 4];      // of q and k
   __shared__ long long kept[kMropeTokens];                      // where a token's first head goes in the pool; below 0: nowhere
   constexpr int HPI = kMropeThreads / LPH, HPW = 32 / LPH;      // heads at once: of the CTA, of a warp
   pdl_trigger();
@@ -246,6 +247,13 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
   };
   load(v[0]);
   load(v[1]);
+  [[maybe_unused]] const float inv_dim = 1.f / static_cast<float>(D);
+  if constexpr (NORM) {
+    if (threadIdx.x < D) {
+      norm_w[0][threadIdx.x] = p.q_norm_w ? __bfloat162float(p.q_norm_w[threadIdx.x]) : 1.f;
+      norm_w[1][threadIdx.x] = p.k_norm_w ? __bfloat162float(p.k_norm_w[threadIdx.x]) : 1.f;
+    }
+  }
   if (threadIdx.x < rows) {
     const long long slot = p.slots[t0 + threadIdx.x], blk = slot / p.block_size;
     kept[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : (blk * p.Hkv * p.block_size + (slot - blk * p.block_size)) * D;
@@ -260,7 +268,7 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
   __syncthreads();
   HeadWalk at(g, heads);
   auto work = [&](Vec (&x)[2]) {
-    float a[W], b[W];
+    alignas(16) float a[W], b[W];
     const bool here = live && at.t < rows;
     const bool is_q = at.s < p.Hq, is_v = at.s >= p.Hq + p.Hkv;
     if (here) {
@@ -269,23 +277,25 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
     }
     load(x);
     if constexpr (NORM) {
-      float ss = 0.f;
+      float2* a2 = reinterpret_cast<float2*>(a);
+      float2* b2 = reinterpret_cast<float2*>(b);
+      float2 sq = make_float2(0.f, 0.f);
       if (here) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) ss += a[i] * a[i] + b[i] * b[i];
+        for (int i = 0; i < W / 2; ++i) sq = __ffma2_rn(b2[i], b2[i], __ffma2_rn(a2[i], a2[i], sq));
       }
+      float ss = sq.x + sq.y;
 #pragma unroll
       for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const __nv_bfloat16* nw = is_q ? p.q_norm_w : (is_v ? nullptr : p.k_norm_w);
-      if (here && nw != nullptr) {                              // (not rounded before the rotation)
-        const float rstd = rsqrtf(ss / D + p.eps);
-        float w[W];
-        MropeVec<W>::widen(*reinterpret_cast<const Vec*>(nw + c0), w);
+      if (here && !is_v && (is_q ? p.q_norm_w : p.k_norm_w) != nullptr) {       // (not rounded before the rotation)
+        const float rstd = rsqrtf(ss * inv_dim + p.eps);
+        const float2 r2 = make_float2(rstd, rstd);
+        const float* w = is_q ? norm_w[0] : norm_w[1];
 #pragma unroll
-        for (int i = 0; i < W; ++i) a[i] *= rstd * w[i];
-        MropeVec<W>::widen(*reinterpret_cast<const Vec*>(nw + c1), w);
-#pragma unroll
-        for (int i = 0; i < W; ++i) b[i] *= rstd * w[i];
+        for (int i = 0; i < W / 2; ++i) {
+          a2[i] = __fmul2_rn(__fmul2_rn(a2[i], r2), *reinterpret_cast<const float2*>(w + c0 + 2 * i));
+          b2[i] = __fmul2_rn(__fmul2_rn(b2[i], r2), *reinterpret_cast<const float2*>(w + c1 + 2 * i));
+        }
       }
     }
     if (here) {
