@@ -8,8 +8,9 @@
 // of the rounded row: what a later reader of the stream would compute. b and the scaled branch are not rounded in between.
 //
 // Bound by memory: x and residual in, h and y out, four rows. The row stays in registers between its reductions (two for rms, three
-// with the mean of a layer norm). Measured (us, of what a copy of these bytes would take): 8192 x 5120 bf16 67 (77 %; 83 with one
-// access per thread and the weights asked for when they are needed), 2000 x 8192 fp32 46 (88 %), one row of 2560 2.2.
+// with the mean of a layer norm). Measured (us, of what a copy of these bytes would take): 8192 x 5120 bf16 64 (79 %; 83 with one
+// access per thread and the weights asked for when they are needed), 8192 x 4096 47 (88 %), 2000 x 8192 fp32 45 (89 %), one row of 2560
+// 2.2; rows of an odd length: 8192 x 5119 143 (241 element by element), 8192 x 1003 26 (32).
 #include "api.h"
 #include "common.cuh"
 #include "typed.cuh"
@@ -80,14 +81,88 @@ struct Pack {
   }
 };
 
-template <typename T, int V, int VPT, int MOST, bool LAYER>
+// Rows that do not start on 16 bytes but all at the same place within 16 bytes (rows of an odd length behind each other) are covered by
+// the aligned vectors that hold them: vector v has the elements v V - o ... of a row that starts o elements behind a boundary. Ends are
+// read and written element by element (what is beyond the row counts as 0 and is not touched).
+template <typename T, int V>
+__device__ __forceinline__ void load_part(Pack<T, V>& d, const T* row, int first, int dim) {
+  if (first >= 0 && first + V <= dim) {
+    d.load(row + first);
+  } else {
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = first + j >= 0 && first + j < dim ? to_f(row[first + j]) : 0.f;
+    d.narrow(f);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_part(const Pack<T, V>& s, T* row, int first, int dim) {
+  if (first >= 0 && first + V <= dim) {
+    s.store(row + first);
+  } else {
+    float f[V];
+    s.widen(f);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (first + j >= 0 && first + j < dim) row[first + j] = from_f<T>(f[j]);
+  }
+}
+// The last O elements of vector a and the first V - O of b.
+template <typename T, int V, int O>
+__device__ __forceinline__ uint4 joined(const uint4& a, const uint4& b) {
+  constexpr int bytes = 16 - O * static_cast<int>(sizeof(T)), q = bytes / 4;
+  const uint32_t w[9] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, 0u};
+  if constexpr (bytes % 4 == 0) return make_uint4(w[q], w[q + 1], w[q + 2], w[q + 3]);
+  else return make_uint4(__funnelshift_r(w[q], w[q + 1], 16), __funnelshift_r(w[q + 1], w[q + 2], 16), __funnelshift_r(w[q + 2], w[q + 3], 16),
+                         __funnelshift_r(w[q + 3], w[q + 4], 16));
+}
+// Elements first .. first + V of a vector of weights that starts on 16 bytes, first = v V - o.
+template <typename T, int V>
+__device__ __forceinline__ void load_shifted(Pack<T, V>& d, const T* w, int v, int o, int dim) {
+  Pack<T, V> a, b;
+  load_part(b, w, v * V, dim);
+  if (o == 0) {
+    d = b;
+    return;
+  }
+  load_part(a, w, (v - 1) * V, dim);
+  switch (o) {
+    case 1: d.w = joined<T, V, 1>(a.w, b.w); break;
+    case 2: d.w = joined<T, V, 2>(a.w, b.w); break;
+    case 3: d.w = joined<T, V, 3>(a.w, b.w); break;
+    default:
+      if constexpr (V == 8) {
+        switch (o) {
+          case 4: d.w = joined<T, V, 4>(a.w, b.w); break;
+          case 5: d.w = joined<T, V, 5>(a.w, b.w); break;
+          case 6: d.w = joined<T, V, 6>(a.w, b.w); break;
+          default: d.w = joined<T, V, 7>(a.w, b.w); break;
+        }
+      }
+  }
+}
+
+template <typename T, int V, int VPT, int MOST, bool LAYER, bool SHIFT>
 __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParams p) {
   __shared__ float red[3][32];
   pdl_trigger();
   pdl_wait();
   const size_t row = blockIdx.x;
-  const int nvec = p.dim / V;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const int o = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)) : 0;
+  const int nvec = SHIFT ? (p.dim + o + V - 1) / V : p.dim / V;
+  auto get = [&](Pack<T, V>& d, const T* from, int v) {
+    if constexpr (SHIFT) load_part(d, from, v * V - o, p.dim);
+    else d.load(from + static_cast<size_t>(v) * V);
+  };
+  auto put = [&](const Pack<T, V>& d, T* to, int v) {
+    if constexpr (SHIFT) store_part(d, to, v * V - o, p.dim);
+    else d.store(to + static_cast<size_t>(v) * V);
+  };
+  auto weights = [&](Pack<T, V>& d, const T* from, int v) {
+    if constexpr (SHIFT) load_shifted(d, from, v, o, p.dim);
+    else d.load(from + static_cast<size_t>(v) * V);
+  };
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
   const T* post = static_cast<const T*>(p.post_w);
   const T* gate = static_cast<const T*>(p.gate);
@@ -99,9 +174,9 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v < nvec) {
-      xv[i].load(x + static_cast<size_t>(v) * V);
-      if (res) rv[i].load(res + static_cast<size_t>(v) * V);
-      if (post) wv[i].load(post + static_cast<size_t>(v) * V);
+      get(xv[i], x, v);
+      if (res) get(rv[i], res, v);
+      if (post) weights(wv[i], post, v);
     }
   }
   float rstd = 1.f;
@@ -132,7 +207,7 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
         for (int j = 0; j < V; ++j) hv[i][j] *= rstd * (f[j] + p.w_bias);
       }
       if (gate) {
-        t.load(gate + static_cast<size_t>(v) * V);
+        weights(t, gate, v);
         t.widen(f);
 #pragma unroll
         for (int j = 0; j < V; ++j) hv[i][j] *= f[j];
@@ -145,7 +220,7 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
         for (int j = 0; j < V; ++j) hv[i][j] += f[j];
       }
       t.narrow(hv[i]);
-      t.store(static_cast<T*>(p.h) + row * p.ldh + static_cast<size_t>(v) * V);
+      put(t, static_cast<T*>(p.h) + row * p.ldh, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) stat += LAYER ? hv[i][j] : hv[i][j] * hv[i][j];
     }
@@ -154,7 +229,7 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    if (v < nvec) wv[i].load(pre + static_cast<size_t>(v) * V);
+    if (v < nvec) weights(wv[i], pre, v);
   }
   float mean = 0.f;
   stat = row_sum(stat, red[1]) / static_cast<float>(p.dim);
@@ -163,9 +238,13 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if (threadIdx.x + i * blockDim.x < nvec) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nvec) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss += (hv[i][j] - mean) * (hv[i][j] - mean);
+        for (int j = 0; j < V; ++j) {
+          const float d = hv[i][j] - mean;
+          if (!SHIFT || static_cast<unsigned>(v * V - o + j) < static_cast<unsigned>(p.dim)) ss += d * d;
+        }
       }
     }
     stat = row_sum(ss, red[2]) / static_cast<float>(p.dim);
@@ -181,20 +260,20 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
 #pragma unroll
       for (int j = 0; j < V; ++j) hv[i][j] = (hv[i][j] - mean) * rstd * (f[j] + p.w_bias);
       if (bias) {
-        t.load(bias + static_cast<size_t>(v) * V);
+        weights(t, bias, v);
         t.widen(f);
 #pragma unroll
         for (int j = 0; j < V; ++j) hv[i][j] += f[j];
       }
       t.narrow(hv[i]);
-      t.store(static_cast<T*>(p.y) + row * p.ldy + static_cast<size_t>(v) * V);
+      put(t, static_cast<T*>(p.y) + row * p.ldy, v);
     }
   }
 }
 
-template <typename T, int V, bool LAYER>
+template <typename T, int V, bool LAYER, bool SHIFT>
 static int launch_branch_norm(const BranchNormParams& p, int rows, cudaStream_t stream) {
-  const int nvec = p.dim / V;
+  const int nvec = SHIFT ? (p.dim + 2 * V - 2) / V : p.dim / V;
   // Few rows: one access per thread, the shortest way through a row. Many rows: several per thread, so that more rows are on an SM and
   // fewer warps meet at a row's barriers.
   int each = 1;
@@ -202,18 +281,29 @@ static int launch_branch_norm(const BranchNormParams& p, int rows, cudaStream_t 
   while (each < most && nvec > 64 * each && rows > 2 * device_sm_count()) each *= 2;
   while (each < 32 / V && nvec > 1024 * each) each *= 2;
   const int threads = ((nvec + each - 1) / each + 31) / 32 * 32;
+  if (threads > 1024) return -1;                            // (a shifted row of the greatest length: left to the form by elements)
   auto run = [&](auto kern) { return static_cast<int>(launch_kernel(kern, dim3(rows), dim3(threads), 0, stream, p)); };
-  if (each == 1) return run(branch_norm_kernel<T, V, 1, 1024, LAYER>);
-  if (each == 2) return threads <= 256 ? run(branch_norm_kernel<T, V, 2, 256, LAYER>) : run(branch_norm_kernel<T, V, 2, 1024, LAYER>);
-  if (each == 4) return threads <= 256 ? run(branch_norm_kernel<T, V, 4, 256, LAYER>) : run(branch_norm_kernel<T, V, 4, 1024, LAYER>);
+  if (each == 1) return run(branch_norm_kernel<T, V, 1, 1024, LAYER, SHIFT>);
+  if (each == 2) return threads <= 256 ? run(branch_norm_kernel<T, V, 2, 256, LAYER, SHIFT>) : run(branch_norm_kernel<T, V, 2, 1024, LAYER, SHIFT>);
+  if (each == 4) return threads <= 256 ? run(branch_norm_kernel<T, V, 4, 256, LAYER, SHIFT>) : run(branch_norm_kernel<T, V, 4, 1024, LAYER, SHIFT>);
   if constexpr (V < 8) {
-    if (each == 8) return threads <= 256 ? run(branch_norm_kernel<T, V, 8, 256, LAYER>) : run(branch_norm_kernel<T, V, 8, 1024, LAYER>);
+    if (each == 8) return threads <= 256 ? run(branch_norm_kernel<T, V, 8, 256, LAYER, SHIFT>) : run(branch_norm_kernel<T, V, 8, 1024, LAYER, SHIFT>);
   }
   if constexpr (V == 1) {
-    if (each == 16) return run(branch_norm_kernel<T, V, 16, 1024, LAYER>);
-    return run(branch_norm_kernel<T, V, 32, 1024, LAYER>);
+    if (each == 16) return run(branch_norm_kernel<T, V, 16, 1024, LAYER, SHIFT>);
+    return run(branch_norm_kernel<T, V, 32, 1024, LAYER, SHIFT>);
   }
   return -1;
+}
+
+template <typename T, int V>
+static int choose_branch_norm(const BranchNormParams& p, int rows, bool layer, bool wide, bool shifted, cudaStream_t stream) {
+  if (wide) return layer ? launch_branch_norm<T, V, true, false>(p, rows, stream) : launch_branch_norm<T, V, false, false>(p, rows, stream);
+  if (shifted) {
+    const int rc = layer ? launch_branch_norm<T, V, true, true>(p, rows, stream) : launch_branch_norm<T, V, false, true>(p, rows, stream);
+    if (rc != -1) return rc;
+  }
+  return layer ? launch_branch_norm<T, 1, true, false>(p, rows, stream) : launch_branch_norm<T, 1, false, false>(p, rows, stream);
 }
 
 }  // namespace mx
@@ -225,15 +315,17 @@ extern "C" int mx_branch_norm(const MxBranchNorm* a, void* stream_) {
   const BranchNormParams p{a->x, a->residual, a->post_w, a->gate, a->pre_w, a->pre_b, a->h, a->y, a->ldx, a->ldr, a->ldh, a->ldy, a->dim, a->scale, a->eps, a->w_bias};
   const int rows = a->rows, dim = a->dim, fp32 = a->fp32, layer_norm = a->layer_norm;
   const int v = fp32 ? 4 : 8;
-  bool wide = dim % v == 0 && a->ldx % v == 0 && a->ldr % v == 0 && a->ldh % v == 0 && a->ldy % v == 0;
-  for (const void* t : {a->x, a->residual, a->post_w, a->gate, a->pre_w, a->pre_b, static_cast<const void*>(a->h), static_cast<const void*>(a->y)})
+  bool wide = dim % v == 0 && a->ldx % v == 0 && a->ldr % v == 0 && a->ldh % v == 0 && a->ldy % v == 0, shifted = true;
+  for (const void* t : {a->post_w, a->gate, a->pre_w, a->pre_b}) shifted = shifted && aligned_to(t, 16);
+  wide = wide && shifted;
+  const uintptr_t place = reinterpret_cast<uintptr_t>(a->x) % 16;
+  auto row_at = [&](const void* t, long long ld) {           // wide: on a boundary; shifted: every row where x's is
+    if (t == nullptr) return;
     wide = wide && aligned_to(t, 16);
+    shifted = shifted && reinterpret_cast<uintptr_t>(t) % 16 == place && (rows == 1 || (ld - a->ldx) % v == 0);
+  };
+  row_at(a->x, a->ldx), row_at(a->residual, a->ldr), row_at(a->h, a->ldh), row_at(a->y, a->ldy);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (fp32) {
-    if (wide) return layer_norm ? launch_branch_norm<float, 4, true>(p, rows, stream) : launch_branch_norm<float, 4, false>(p, rows, stream);
-    return layer_norm ? launch_branch_norm<float, 1, true>(p, rows, stream) : launch_branch_norm<float, 1, false>(p, rows, stream);
-  }
-  if (wide)
-    return layer_norm ? launch_branch_norm<__nv_bfloat16, 8, true>(p, rows, stream) : launch_branch_norm<__nv_bfloat16, 8, false>(p, rows, stream);
-  return layer_norm ? launch_branch_norm<__nv_bfloat16, 1, true>(p, rows, stream) : launch_branch_norm<__nv_bfloat16, 1, false>(p, rows, stream);
+  return fp32 ? choose_branch_norm<float, 4>(p, rows, layer_norm != 0, wide, shifted, stream)
+              : choose_branch_norm<__nv_bfloat16, 8>(p, rows, layer_norm != 0, wide, shifted, stream);
 }
