@@ -47,37 +47,42 @@ struct MropeParams {
   float eps, mscale;
 };
 
-// Codes of 64 values (two per lane): q = round((x - low) / scale), scale = (high - low) / levels, both kept in bf16.
+// The step and offset of 64 values between mn and mx as they are stored (bf16), and a value's code: round((x - low) / scale). Codes are
+// taken against the rounded pair, which is what a reader expands them with.
+template <int BITS>
+struct KvCode {
+  static constexpr int kTop = BITS == 8 ? 255 : 15;
+  float scale, low;
+  __device__ __forceinline__ KvCode(float mn, float mx)
+      : scale(__bfloat162float(__float2bfloat16((mx - mn) / static_cast<float>(kTop)))), low(__bfloat162float(__float2bfloat16(mn))) {
+    if (scale == 0.f) scale = 1.f;
+  }
+  __device__ __forceinline__ uint32_t operator()(float x) const { return static_cast<uint32_t>(min(kTop, max(0, __float2int_rn((x - low) / scale)))); }
+  __device__ __forceinline__ uint32_t meta() const { return pack_bf16(scale, low); }
+};
+
+// Codes of 64 values, two per lane.
 template <int BITS>
 __device__ __forceinline__ void store_codes(float a, float b, int lane, uint8_t* dst, __nv_bfloat16* meta) {
-  constexpr float kLevels = BITS == 8 ? 255.f : 15.f;
   float mn = fminf(a, b), mx = fmaxf(a, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
-  // codes are taken against the rounded pair, which is what a reader expands them with
-  float scale = __bfloat162float(__float2bfloat16((mx - mn) / kLevels));
-  const float low = __bfloat162float(__float2bfloat16(mn));
-  if (scale == 0.f) scale = 1.f;
-  const int top = static_cast<int>(kLevels);
-  const int qa = min(top, max(0, __float2int_rn((a - low) / scale)));
-  const int qb = min(top, max(0, __float2int_rn((b - low) / scale)));
+  const KvCode<BITS> code(mn, mx);
+  const uint32_t qa = code(a), qb = code(b);
   if constexpr (BITS == 8) {
     dst[lane] = static_cast<uint8_t>(qa);
     dst[32 + lane] = static_cast<uint8_t>(qb);
   } else {                                                        // neighbouring lanes share a byte, the even one in the low half
-    const int qa1 = __shfl_down_sync(0xffffffffu, qa, 1), qb1 = __shfl_down_sync(0xffffffffu, qb, 1);
+    const uint32_t qa1 = __shfl_down_sync(0xffffffffu, qa, 1), qb1 = __shfl_down_sync(0xffffffffu, qb, 1);
     if ((lane & 1) == 0) {
       dst[lane >> 1] = static_cast<uint8_t>(qa | (qa1 << 4));
       dst[16 + (lane >> 1)] = static_cast<uint8_t>(qb | (qb1 << 4));
     }
   }
-  if (lane == 0) {
-    meta[0] = __float2bfloat16(scale);
-    meta[1] = __float2bfloat16(low);
-  }
+  if (lane == 0) *reinterpret_cast<uint32_t*>(meta) = code.meta();
 }
 
 // Any head size up to 256, any rotated width, every pool. A CTA is one token, a warp one head at a time, staged in shared memory.
@@ -220,12 +225,23 @@ struct HeadWalk {
   }
 };
 
-template <int W, int LPH, bool NORM>
+// Eight values' codes as they are stored: 8 bytes, or 4 with the first of two in the low half of a byte.
+template <int BITS>
+__device__ __forceinline__ void store_eight(const float (&x)[8], const KvCode<BITS>& code, uint8_t* dst) {
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[BITS == 8 ? i / 4 : 0] |= code(x[i]) << (BITS == 8 ? i % 4 * 8 : i * 4);
+  if constexpr (BITS == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = w[0];
+}
+
+// BITS 8 and 4 (W = 8): 64 columns are those of four lanes, or (halves 64 or a multiple apart) one vector of eight lanes each.
+template <int W, int LPH, bool NORM, int BITS>
 __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_vec_kernel(const MropeParams p, int tokens, int per_block) {
   using Vec = typename MropeVec<W>::type;
   __shared__ __align__(16) float cs[kMropeTokens * kMropeMaxDim / 2], sn[kMropeTokens * kMropeMaxDim / 2];
   __shared__ __align__(16) float norm_w[NORM ? 2 : 1][NORM ? kMropeMaxDim : 4];      // of q and k
-  __shared__ long long kept[kMropeTokens];                      // where a token's first head goes in the pool; below 0: nowhere
+  __shared__ long long kept[kMropeTokens];                      // the row of a token's first head in the pool; below 0: nowhere
   constexpr int HPI = kMropeThreads / LPH, HPW = 32 / LPH;      // heads at once: of the CTA, of a warp
   pdl_trigger();
   pdl_wait();
@@ -234,7 +250,6 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
   int c0, c1;
   const bool turns = unit_columns<W>(u, half, p.pairs, c0, c1), live = u * 2 * W < D;
   const __nv_bfloat16* src = p.qkv + t0 * p.ldqkv;
-  const long long page_head = static_cast<long long>(p.block_size) * D;
   Vec v[2][2];
   HeadWalk ahead(g, heads);
   auto load = [&](Vec (&x)[2]) {
@@ -256,7 +271,7 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
   }
   if (threadIdx.x < rows) {
     const long long slot = p.slots[t0 + threadIdx.x], blk = slot / p.block_size;
-    kept[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : (blk * p.Hkv * p.block_size + (slot - blk * p.block_size)) * D;
+    kept[threadIdx.x] = slot < 0 || slot >= p.n_slots ? -1 : blk * p.Hkv * p.block_size + (slot - blk * p.block_size);
   }
   for (int i = threadIdx.x; i < rows * half; i += kMropeThreads) {
     const int t = i / half;
@@ -298,18 +313,48 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
         }
       }
     }
-    if (here) {
-      if (turns && !is_v) turn_unit<W>(a, b, cs + at.t * half + W * u, sn + at.t * half + W * u, p.pairs);
-      __nv_bfloat16* dst = nullptr;
-      if (is_q) {
-        dst = p.q_out + (t0 + at.t) * p.ldq + at.s * D;
-      } else if (kept[at.t] >= 0) {                             // (a row without a slot leaves the pool alone)
-        const int head = at.s - p.Hq - (is_v ? p.Hkv : 0);
-        dst = static_cast<__nv_bfloat16*>(is_v ? p.v_pool : p.k_pool) + kept[at.t] + head * page_head;
-      }
-      if (dst != nullptr) {
-        *reinterpret_cast<Vec*>(dst + c0) = MropeVec<W>::narrow(a);
-        *reinterpret_cast<Vec*>(dst + c1) = MropeVec<W>::narrow(b);
+    if (here && turns && !is_v) turn_unit<W>(a, b, cs + at.t * half + W * u, sn + at.t * half + W * u, p.pairs);
+    const int head = at.s - p.Hq - (is_v ? p.Hkv : 0);
+    const long long row = here && !is_q ? kept[at.t] : -1;                 // (a row without a slot leaves the pool alone)
+    const long long place = row + static_cast<long long>(head) * p.block_size;
+    __nv_bfloat16* dst = nullptr;
+    if (here && is_q) dst = p.q_out + (t0 + at.t) * p.ldq + at.s * D;
+    else if (BITS == 16 && row >= 0) dst = static_cast<__nv_bfloat16*>(is_v ? p.v_pool : p.k_pool) + place * D;
+    if (dst != nullptr) {
+      *reinterpret_cast<Vec*>(dst + c0) = MropeVec<W>::narrow(a);
+      *reinterpret_cast<Vec*>(dst + c1) = MropeVec<W>::narrow(b);
+    }
+    if constexpr (BITS != 16) {
+      if (__any_sync(0xffffffffu, row >= 0)) {
+        const bool apart = (c0 >> 6) != (c1 >> 6);
+        float low[2], high[2];
+        low[0] = high[0] = here ? a[0] : 0.f;
+        low[1] = high[1] = here ? b[0] : 0.f;
+        if (here) {
+#pragma unroll
+          for (int i = 1; i < W; ++i) {
+            low[0] = fminf(low[0], a[i]), high[0] = fmaxf(high[0], a[i]);
+            low[1] = fminf(low[1], b[i]), high[1] = fmaxf(high[1], b[i]);
+          }
+        }
+        if (!apart) low[0] = low[1] = fminf(low[0], low[1]), high[0] = high[1] = fmaxf(high[0], high[1]);
+#pragma unroll
+        for (int o = 1; o <= 4; o <<= 1) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float l = __shfl_xor_sync(0xffffffffu, low[i], o), h = __shfl_xor_sync(0xffffffffu, high[i], o);
+            if (o < 4 || apart) low[i] = fminf(low[i], l), high[i] = fmaxf(high[i], h);
+          }
+        }
+        if (row >= 0) {
+          const KvCode<BITS> code_a(low[0], high[0]), code_b(low[1], high[1]);
+          uint8_t* codes = static_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + place * (D * BITS / 8);
+          store_eight<BITS>(a, code_a, codes + c0 * BITS / 8);
+          store_eight<BITS>(b, code_b, codes + c1 * BITS / 8);
+          uint32_t* meta = reinterpret_cast<uint32_t*>(is_v ? p.v_meta : p.k_meta) + place * (D / 64);
+          if (u % (apart ? 8 : 4) == 0) meta[c0 >> 6] = code_a.meta();
+          if (apart && u % 8 == 0) meta[c1 >> 6] = code_b.meta();
+        }
       }
     }
     at.step(HPI, heads);
@@ -446,23 +491,30 @@ extern "C" int mx_mrope_append(const MxMropeAppend* a, void* stream_) {
   cudaError_t e;
   auto bits_of = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
   // Accesses of 8 bytes leave room for more warps, those of 16 bytes take fewer instructions: 1031 tokens of 32 + 4 heads 8.1 us against 10.8,
-  // 8191 of 64 + 16 heads with norms 81 against 73.
-  const int w = kv_bits == 16 ? mrope_width(mrope_tokens(T) == kMropeTokens ? 8 : 4, D, rot_dim, bits_of(a->qkv) | bits_of(a->q_out) | bits_of(a->k_pool) | bits_of(a->v_pool) | bits_of(a->q_norm_w) |
-                                            bits_of(a->k_norm_w), a->ldqkv | a->ldq) : 0;
+  // 8191 of 64 + 16 heads with norms 81 against 73. Codes are made of 8 values of a lane at once.
+  const bool coded = kv_bits != 16;
+  int w = mrope_width(coded || mrope_tokens(T) == kMropeTokens ? 8 : 4, D, rot_dim, bits_of(a->qkv) | bits_of(a->q_out) | bits_of(a->q_norm_w) | bits_of(a->k_norm_w) |
+                      (coded ? 0 : bits_of(a->k_pool) | bits_of(a->v_pool)), a->ldqkv | a->ldq);
+  if (coded && (w != 8 || !(a->pairs || rot_dim <= 64 || rot_dim % 128 == 0) || (bits_of(a->k_pool) | bits_of(a->v_pool)) % 8 ||
+                (bits_of(a->k_meta) | bits_of(a->v_meta)) % 4))
+    w = 0;
   if (w != 0) {
     const int lanes = D / (2 * w), per = mrope_tokens(T), blocks = (T + per - 1) / per;
     const bool norm = a->q_norm_w != nullptr || a->k_norm_w != nullptr;
-#define MX_MROPE(W_, L_)                                                                                                          \
-    e = norm ? launch_kernel(mrope_append_vec_kernel<W_, L_, true>, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)      \
-             : launch_kernel(mrope_append_vec_kernel<W_, L_, false>, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)
-    if (w == 8 && lanes <= 4) MX_MROPE(8, 4);
-    else if (w == 8 && lanes <= 8) MX_MROPE(8, 8);
-    else if (w == 8) MX_MROPE(8, 16);
-    else if (lanes <= 8) MX_MROPE(4, 8);
-    else if (lanes <= 16) MX_MROPE(4, 16);
-    else MX_MROPE(4, 32);
+    auto run = [&](auto kern) { return static_cast<int>(launch_kernel(kern, dim3(blocks), dim3(kMropeThreads), 0, stream, p, T, per)); };
+#define MX_MROPE(W_, L_, B_) return norm ? run(mrope_append_vec_kernel<W_, L_, true, B_>) : run(mrope_append_vec_kernel<W_, L_, false, B_>)
+#define MX_MROPE_LANES(B_)              \
+  if (lanes <= 4) MX_MROPE(8, 4, B_);   \
+  if (lanes <= 8) MX_MROPE(8, 8, B_);   \
+  MX_MROPE(8, 16, B_)
+    if (kv_bits == 8) { MX_MROPE_LANES(8); }
+    if (kv_bits == 4) { MX_MROPE_LANES(4); }
+    if (w == 8) { MX_MROPE_LANES(16); }
+    if (lanes <= 8) MX_MROPE(4, 8, 16);
+    if (lanes <= 16) MX_MROPE(4, 16, 16);
+    MX_MROPE(4, 32, 16);
+#undef MX_MROPE_LANES
 #undef MX_MROPE
-    return static_cast<int>(e);
   }
   if (kv_bits == 16) e = launch_kernel(mrope_append_kernel<16>, dim3(T), dim3(kMropeThreads), 0, stream, p);
   else if (kv_bits == 8) e = launch_kernel(mrope_append_kernel<8>, dim3(T), dim3(kMropeThreads), 0, stream, p);

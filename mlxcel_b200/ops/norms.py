@@ -13,6 +13,15 @@ _ARGS = struct.Struct("PqPqPPPPPqPqiifffii")        # MxBranchNorm of csrc/api.h
 _TYPES = (torch.bfloat16, torch.float32)
 
 
+def _row_stride(t: torch.Tensor | None, rows: int, dim: int) -> int:
+    if t is None:
+        return dim
+    ld, one = t.stride()
+    if one != 1 and dim > 1 or rows > 1 and ld < dim:
+        raise ValueError("the elements of a row have to be adjacent and rows apart")
+    return ld
+
+
 def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w: torch.Tensor | None = None,
                 gate: torch.Tensor | None = None, scale: float = 1.0, pre_w: torch.Tensor | None = None,
                 pre_b: torch.Tensor | None = None, layer_norm: bool = False, eps: float = 1e-6, w_bias: float = 0.0,
@@ -30,12 +39,12 @@ def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w
     dtype, dev = x.dtype, x.get_device()
     if dtype not in _TYPES:
         raise ValueError(f"branch_norm takes bf16 or fp32 rows, not {dtype}")
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != dev):
-            raise ValueError(f"{name} has to be like x: {tuple(shape)} {dtype} on {x.device}")
-    for name, t in (("post_w", post_w), ("gate", gate), ("pre_w", pre_w), ("pre_b", pre_b)):
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype or residual.get_device() != dev) or (
+            out is not None and (out.shape != shape or out.dtype != dtype or out.get_device() != dev)):
+        raise ValueError(f"residual and out have to be like x: {tuple(shape)} {dtype} on {x.device}")
+    for t in (post_w, gate, pre_w, pre_b):
         if t is not None and (t.dtype != dtype or t.dim() != 1 or t.numel() != dim or t.get_device() != dev or not t.is_contiguous()):
-            raise ValueError(f"{name} has to be a contiguous [{dim}] {dtype} tensor on {x.device}")
+            raise ValueError(f"weights, gate and bias have to be contiguous [{dim}] {dtype} tensors on {x.device}")
     if pre_b is not None and (pre_w is None or not layer_norm):
         raise ValueError("pre_b belongs to a layer norm (pre_w, layer_norm=True)")
     if not 1 <= dim <= 32768:
@@ -43,19 +52,13 @@ def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w
     if not x.is_cuda:
         y, h = ref.branch_norm(x, residual, post_w, gate, scale, pre_w, pre_b, layer_norm, eps, w_bias)
         return y, h if out is None else out.copy_(h)
-    strides = []
-    for name, t in (("x", x), ("residual", residual), ("out", out)):
-        ld = dim
-        if t is not None:
-            ld, one = t.stride()
-            if one != 1 and dim > 1 or rows > 1 and ld < dim:
-                raise ValueError(f"the elements of a row of {name} have to be adjacent and its rows apart")
-        strides.append(ld)
-    h = torch.empty(shape, dtype=dtype, device=x.device) if out is None else out
-    y = torch.empty(shape, dtype=dtype, device=x.device) if pre_w is not None else None
+    dense = x.is_contiguous()
+    ldx, ldr, ldh = (_row_stride(t, rows, dim) for t in (x, residual, out))
+    h = out if out is not None else torch.empty_like(x) if dense else torch.empty(shape, dtype=dtype, device=x.device)
+    y = None if pre_w is None else torch.empty_like(x) if dense else torch.empty(shape, dtype=dtype, device=x.device)
     if rows:
         at = lambda t: 0 if t is None else t.data_ptr()    # noqa: E731
         _lib.launch_on(x.device, "mx_branch_norm", _ARGS.pack(
-            x.data_ptr(), strides[0], at(residual), strides[1], at(post_w), at(gate), at(pre_w), at(pre_b), h.data_ptr(), strides[2], at(y), dim,
+            x.data_ptr(), ldx, at(residual), ldr, at(post_w), at(gate), at(pre_w), at(pre_b), h.data_ptr(), ldh, at(y), dim,
             rows, dim, scale, eps, w_bias, layer_norm, dtype == torch.float32))
     return y, h
