@@ -187,15 +187,24 @@ __device__ __forceinline__ bool unit_columns(int u, int half, int pairs, int& c0
   }
   return turns;
 }
-// Turns a lane's 2 W values by the W angles from cs, sn on (which carry the scale).
+// Rows of n floats that lanes read W at a time are kept so that a warp's accesses of 16 bytes are neighbours: with W = 8 the first four
+// of every eight, then the others.
 template <int W>
-__device__ __forceinline__ void turn_unit(float (&a)[W], float (&b)[W], const float* cs, const float* sn, int pairs) {
-  float c[W], s[W];
+__device__ __forceinline__ int kept_at(int i, int n) {
+  return W == 8 ? (i >> 2 & 1) * (n >> 1) + (i >> 3) * 4 + (i & 3) : i;
+}
+template <int W>
+__device__ __forceinline__ void read_kept(float (&d)[W], const float* row, int first, int n) {
 #pragma unroll
-  for (int i = 0; i < W; i += 4) {
-    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + i);
-    *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(sn + i);
-  }
+  for (int i = 0; i < W; i += 4) *reinterpret_cast<float4*>(d + i) = *reinterpret_cast<const float4*>(row + kept_at<W>(first + i, n));
+}
+
+// Turns a lane's 2 W values by its W angles (from W u on, of `half`; they carry the scale).
+template <int W>
+__device__ __forceinline__ void turn_unit(float (&a)[W], float (&b)[W], const float* cs, const float* sn, int u, int half, int pairs) {
+  alignas(16) float c[W], s[W];
+  read_kept<W>(c, cs, W * u, half);
+  read_kept<W>(s, sn, W * u, half);
   if (pairs) {
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) {
@@ -265,8 +274,9 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
   [[maybe_unused]] const float inv_dim = 1.f / static_cast<float>(D);
   if constexpr (NORM) {
     if (threadIdx.x < D) {
-      norm_w[0][threadIdx.x] = p.q_norm_w ? __bfloat162float(p.q_norm_w[threadIdx.x]) : 1.f;
-      norm_w[1][threadIdx.x] = p.k_norm_w ? __bfloat162float(p.k_norm_w[threadIdx.x]) : 1.f;
+      const int to = kept_at<W>(threadIdx.x, D);
+      norm_w[0][to] = p.q_norm_w ? __bfloat162float(p.q_norm_w[threadIdx.x]) : 1.f;
+      norm_w[1][to] = p.k_norm_w ? __bfloat162float(p.k_norm_w[threadIdx.x]) : 1.f;
     }
   }
   if (threadIdx.x < rows) {
@@ -277,8 +287,9 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
     const int t = i / half;
     float sine, cosine;
     axis_angle(p.ang, t0 + t, i - t * half, sine, cosine);
-    sn[i] = sine * p.mscale;
-    cs[i] = cosine * p.mscale;
+    const int to = t * half + kept_at<W>(i - t * half, half);
+    sn[to] = sine * p.mscale;
+    cs[to] = cosine * p.mscale;
   }
   __syncthreads();
   HeadWalk at(g, heads);
@@ -305,15 +316,17 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) mrope_append_ve
       if (here && !is_v && (is_q ? p.q_norm_w : p.k_norm_w) != nullptr) {       // (not rounded before the rotation)
         const float rstd = rsqrtf(ss * inv_dim + p.eps);
         const float2 r2 = make_float2(rstd, rstd);
-        const float* w = is_q ? norm_w[0] : norm_w[1];
+        alignas(16) float w[W];
+        const float2* w2 = reinterpret_cast<const float2*>(w);
+        read_kept<W>(w, norm_w[is_q ? 0 : 1], c0, D);
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i) {
-          a2[i] = __fmul2_rn(__fmul2_rn(a2[i], r2), *reinterpret_cast<const float2*>(w + c0 + 2 * i));
-          b2[i] = __fmul2_rn(__fmul2_rn(b2[i], r2), *reinterpret_cast<const float2*>(w + c1 + 2 * i));
-        }
+        for (int i = 0; i < W / 2; ++i) a2[i] = __fmul2_rn(__fmul2_rn(a2[i], r2), w2[i]);
+        read_kept<W>(w, norm_w[is_q ? 0 : 1], c1, D);
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) b2[i] = __fmul2_rn(__fmul2_rn(b2[i], r2), w2[i]);
       }
     }
-    if (here && turns && !is_v) turn_unit<W>(a, b, cs + at.t * half + W * u, sn + at.t * half + W * u, p.pairs);
+    if (here && turns && !is_v) turn_unit<W>(a, b, cs + at.t * half, sn + at.t * half, u, half, p.pairs);
     const int head = at.s - p.Hq - (is_v ? p.Hkv : 0);
     const long long row = here && !is_q ? kept[at.t] : -1;                 // (a row without a slot leaves the pool alone)
     const long long place = row + static_cast<long long>(head) * p.block_size;
@@ -439,8 +452,8 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) axial_rope_vec_
     MropeVec<W>::widen(x[0], a);
     MropeVec<W>::widen(x[1], b);
     load(x);
-    const int part = (now.at.s >= p.H) + (now.at.s >= 2 * p.H), h = now.at.s - part * p.H, angle = now.at.t * half + W * now.u;
-    if (part < 2) turn_unit<W>(a, b, cs + angle, sn + angle, 0);
+    const int part = (now.at.s >= p.H) + (now.at.s >= 2 * p.H), h = now.at.s - part * p.H, angles = now.at.t * half;
+    if (part < 2) turn_unit<W>(a, b, cs + angles, sn + angles, now.u, half, 0);
     float* dst = (part == 0 ? p.q : part == 1 ? p.k : p.v) + (h * p.rows + t0 + now.at.t) * D + W * now.u;
 #pragma unroll
     for (int i = 0; i < W; i += 4) {

@@ -15,6 +15,7 @@ _ARGS = struct.Struct("PqPPPPPPPiiiiiiiff")        # MxTokenLogprobs of csrc/api
 # memory, and the smaller tiles of `linear` are the faster ones. us on the chip / through memory: 8 rows, 128256 x 4096 217 / 171, 64
 # rows 210 / 191, 100 rows 215 / 222, 256 rows 244 / 480; 8 rows, 50257 x 1024 49 / 61, 5000 x 512 27 / 59.
 FEW_ROWS, LARGE_WEIGHTS = 64, 1 << 28
+PARTIAL_BYTES = 256 << 20        # of the column tiles' sums that are held at once
 
 
 class TokenLogprobs(NamedTuple):
@@ -68,8 +69,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, bia
 
 def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: torch.Tensor | None = None, scale: float = 1.0,
                   softcap: float = 0.0) -> TokenLogprobs:
-    """:func:`token_logprobs` (without alternatives) of the logits ``x @ w^T``, which are fp32 and never rounded. ``x`` [R, K] and
-    the head's weights ``w`` [V, K] are bf16 (or both fp32); ``ids`` [R]."""
+    """:func:`token_logprobs` (without alternatives) of the logits ``x @ w^T``, which are fp32 sums and never rounded to fewer bits.
+    ``x`` [R, K] and the head's weights ``w`` [V, K] are bf16 (or both fp32); ``ids`` [R]."""
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
         raise ValueError("hidden rows [R, K] and head weights [V, K] of one type are needed on one device")
     if x.dtype not in (torch.bfloat16, torch.float32):
@@ -86,13 +87,16 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: 
     r = TokenLogprobs(torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, **f), torch.empty(R, 0, dtype=torch.int32, device=x.device),
                       torch.empty(R, 0, **f))
     K = x.shape[1]
-    if R and (R > FEW_ROWS or V * K <= LARGE_WEIGHTS) and x.dtype == torch.bfloat16 and not (K % 8 or x.stride(0) % 8 or w.stride(0) % 8 or (x.data_ptr() | w.data_ptr()) % 16):
-        partials = torch.empty(3 * (-(-V // 256)) + 1, R, **f)
-        ids = ids.contiguous()
-        _lib.launch_on(x.device, "mx_head_logprobs", x.data_ptr(), w.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), _lib.ptr(bias),
-                       int(bias is not None and bias.dtype == torch.float32), float(scale), float(softcap), partials.data_ptr(),
-                       r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), R, V, K, x.stride(0), w.stride(0),
-                       _lib.workspace(x.device).data_ptr())
+    ldx, ldw = x.stride(0) if R > 1 else K, w.stride(0) if V > 1 else K
+    if R and (R > FEW_ROWS or V * K <= LARGE_WEIGHTS) and x.dtype == torch.bfloat16 and not (K % 8 or ldx % 8 or ldw % 8 or (x.data_ptr() | w.data_ptr()) % 16):
+        tiles, ids = -(-V // 256), ids.contiguous()
+        part = min(R, max(256, PARTIAL_BYTES // (12 * tiles) // 256 * 256))
+        partials = torch.empty((3 * tiles + 1) * part, **f)
+        for r0 in range(0, R, part):
+            _lib.launch_on(x.device, "mx_head_logprobs", x.data_ptr() + 2 * r0 * ldx, w.data_ptr(), ids.data_ptr() + r0 * ids.element_size(),
+                           int(ids.dtype == torch.int64), _lib.ptr(bias), int(bias is not None and bias.dtype == torch.float32), float(scale),
+                           float(softcap), partials.data_ptr(), r.logprob.data_ptr() + 4 * r0, r.entropy.data_ptr() + 4 * r0,
+                           r.lse.data_ptr() + 4 * r0, min(part, R - r0), V, K, ldx, ldw, _lib.workspace(x.device).data_ptr())
         return r
     part = max(1, (1 << 26) // V)                 # rows whose logits are held at once: 256 MB
     if R == 0:

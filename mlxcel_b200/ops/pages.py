@@ -20,7 +20,8 @@ def _list(ids) -> list:
 class PageSlabs:
     """The slabs of a pool, [pages, ...] each, in the order in which a buffer holds them. Page ids are host lists (or CPU tensors and
     arrays) and are checked: a page outside the pool, a destination named twice or a source missing raises ``ValueError`` and moves
-    nothing. Slabs whose pages are empty are left out."""
+    nothing. Slabs whose pages are empty are left out. The ids of small calls (106 copies, 320 pages) travel with the launch, which can
+    be captured into a graph; longer tables are copied to the device first, which cannot."""
 
     def __init__(self, slabs: list[torch.Tensor]):
         if not slabs:

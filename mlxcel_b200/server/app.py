@@ -514,7 +514,8 @@ def create_app(state: ServerState) -> FastAPI:
             from ..ops.logprobs import MAX_TOP
             eng = state.worker.engine
             # alternatives at every place of the prompt: ``top_logprobs``, or the count that ``logprobs`` gives
-            many = int(body.get("logprobs") or 0) if not isinstance(body.get("logprobs"), bool) else 0
+            many = body.get("logprobs")
+            many = many if isinstance(many, int) and not isinstance(many, bool) else 0
             many = min(max(0, sp.top_logprobs or many), MAX_TOP, eng.cfg.vocab_size)
             scores = await asyncio.get_running_loop().run_in_executor(
                 None, lambda: sequence_scores(eng.model, eng.cfg, ids, eng.ecfg.block_size, top=many))

@@ -478,6 +478,20 @@ def test_token_logprobs_strided_rows_ids_and_transforms():
     assert r.logprob.shape == (0,) and r.top_ids.shape == (0, 4)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_logprobs_many_of_the_largest_in_few_threads(dtype):
+    """Large values only where the first 126 of a row's 256 threads look (vectors of 16 bytes, thread after thread): more of them than
+    candidates are kept, with and without ties."""
+    E, V, R = 16 // dtype.itemsize, 40000, 150
+    j = torch.arange(V, device=DEV)
+    for values in (torch.rand(R, V, device=DEV) * 50 + 100, torch.full((R, V), 100.0, device=DEV), (j % 97).float().expand(R, V) + 100):
+        x = torch.where((j // E % 256 < 126)[None], values, _rn(R, V, seed=1, dtype=torch.float32)).to(dtype)
+        for top in (5, 64):
+            _check_scores(x, torch.randint(0, V, (R,)).to(DEV), top)
+    one = x[:1].repeat(1, 4)[:, :151936].contiguous()                          # one row in parts
+    _check_scores(one, torch.zeros(1, dtype=torch.long, device=DEV), 64)
+
+
 def test_token_logprobs_repeat_bit_for_bit():
     x = _rn(3, 151936, seed=5, dtype=torch.bfloat16)
     ids = torch.zeros(3, dtype=torch.long, device=DEV)
@@ -538,6 +552,21 @@ def test_head_logprobs_transforms_and_layouts(R):
     _check_head(shifted, w, ids)
     r = logprobs.head_logprobs(x[:0], w, ids[:0])
     assert r.logprob.shape == r.entropy.shape == (0,)
+
+
+def test_head_logprobs_in_parts_and_single_rows(monkeypatch):
+    x, w = _rn(1500, 128, seed=1), _rn(900, 128, seed=2, scale=0.2)
+    ids = torch.randint(0, 900, (1500,)).to(DEV)
+    whole = logprobs.head_logprobs(x, w, ids)
+    monkeypatch.setattr(logprobs, "PARTIAL_BYTES", 1)
+    parts = logprobs.head_logprobs(x, w, ids)
+    assert all(torch.equal(a, b) for a, b in zip(whole[:3], parts[:3]))
+    one = x[3].as_strided((1, 128), (0, 1))                                      # (a row stride of 0)
+    assert one.stride(0) == 0
+    r = logprobs.head_logprobs(one, w, ids[3:4])
+    assert all(torch.allclose(a[0], b[3], atol=1e-5) for a, b in zip(r[:3], whole[:3]))
+    r = logprobs.head_logprobs(x, w[:1], ids * 0)                                # one token: certain
+    assert not r.logprob.any() and not r.entropy.any()
 
 
 def test_head_logprobs_masked_by_bias_and_bad_rows():
