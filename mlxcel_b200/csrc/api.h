@@ -323,7 +323,7 @@ typedef struct MxTokenLogprobs {
 } MxTokenLogprobs;
 int mx_token_logprobs(const MxTokenLogprobs* args, void* stream);
 // The same without alternatives for the logits x[M, K] @ w[V, K]^T (bf16, fp32 sums), which are not stored. partials: fp32
-// [3 * ceil(V / 256) + 1, M]; status: the device status word of bounded waits. -10: strides or addresses that TMA does not take.
+// [6 * ceil(V / 256) + 1, M]; status: the device status word of bounded waits. -10: strides or addresses that TMA does not take.
 int mx_head_logprobs(const void* x, const void* w, const void* ids, int ids64, const void* bias, int bias_fp32, float scale,
                      float softcap, float* partials, float* logprob, float* entropy, float* lse, int M, int V, int K, int ldx,
                      int ldw, void* status, void* stream);

@@ -2,13 +2,14 @@
 // z = x[M, K] @ w[V, K]^T (+ bias), scaled and soft-capped, for each row lse = log sum e^z, log p(id) = z_id - lse, H = lse - sum p z.
 //
 // The products run as in gemm_pair.cu: 256 x 256 tiles on pairs of SMs, operands by TMA, accumulators in TMEM, double-buffered. The
-// epilogue leaves a tile as the sums of its 256 columns per row (m, s, t of logprobs.cuh) in place of 256 logits, and the row's own
-// token's logit where the tile holds it. A second launch joins the column tiles of each row.
+// epilogue leaves a tile as the sums of its columns per row (m, s, t of logprobs.cuh, one set per half of the tile) in place of 256
+// logits, and the row's own token's logit where the tile holds it. A second launch joins the column tiles of each row.
 // Logits of 2047 rows over 128256 tokens would be 1 GB of fp32; what is written instead is 12 MB. The logits are never rounded.
 //
 // Bound by the tensor cores under the power cap: a tile's products take 8 K cycles an SM, its epilogue about 3000 beside them, whose
-// instructions cost power and with it clock. Measured, in a row (us): 2047 rows, K 4096, V 128256 1770 (1.21 PFLOP/s; 1910 with the
-// changes of SHAPED made in any case); the same product by gemm_pair.cu, which writes 525 MB of bf16 logits, 1750, by cuBLAS 1550.
+// instructions cost power and with it clock. Measured, in a row (us): 2047 rows, K 4096, V 128256 1870 (1.15 PFLOP/s); 1790 with the sums
+// left in the tensor core over all of K (3e-6 from the 64-bit result in place of 7e-7), 1910 with the changes of SHAPED made in any
+// case; the same product by gemm_pair.cu, which writes 525 MB of bf16 logits, 1750, by cuBLAS 1550.
 #include <cooperative_groups.h>
 
 #include "api.h"
@@ -18,12 +19,19 @@
 
 namespace mx {
 
+// The tensor core truncates its fp32 sums, which draws every logit towards 0: by 4e-6 of it over K = 4096. Its sums are therefore taken
+// out every 1024 of K and added up, rounded, in the epilogue's registers (128 columns of a row per thread, hence eight warps).
+constexpr int kHlSegment = 1024 / kGpBK;             // K slices of a sum
+constexpr int kHlWarps = 8;                          // of the epilogue
+constexpr int kHlCols = 128;                         // columns of a thread: half a tile
+constexpr int kHlThreads = 64 + 32 * kHlWarps;
+
 bool make_tensor_map_bf16(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols);
 
 struct HeadParams {
   const void* ids;
   const void* bias;
-  float* partials;          // [tiles_n][3][M], then the rows' own logits [M]
+  float* partials;          // [2 tiles_n][3][M], then the rows' own logits [M]
   float* logprob;
   float* entropy;
   float* lse;
@@ -38,7 +46,7 @@ __device__ __forceinline__ long long head_id(const HeadParams& p, int m) {
 
 // SHAPED: the products are not the logits yet (a bias, a scale or a soft cap).
 template <bool SHAPED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGpThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHlThreads, 1)
 head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
   extern __shared__ uint8_t hl_smem[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(hl_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -73,7 +81,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 8);                   // four epilogue warps of each CTA
+      mbar_init(&tmem_empty[a], 2 * kHlWarps);        // the epilogue warps of both CTAs
     }
     fence_mbar_init();
   }
@@ -118,96 +126,111 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int t = pair; ok && t < tiles; t += pairs) {
-        if (!gp_wait(&tmem_empty[acc], acc_phase ^ 1u, p.status, kErrMmaWaitTmem)) break;
-        tc_fence_after_sync();
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!gp_wait(&full_bar[stage], phase, p.status, kErrMmaWaitFull)) {
+        for (int kb0 = 0; ok && kb0 < num_kb; kb0 += kHlSegment) {
+          if (!gp_wait(&tmem_empty[acc], acc_phase ^ 1u, p.status, kErrMmaWaitTmem)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t sa = smem_u32(ring + stage * kGpStageBytes), sb = sa + kGpHalf;
+          for (int kb = kb0; kb < min(num_kb, kb0 + kHlSegment); ++kb) {
+            if (!gp_wait(&full_bar[stage], phase, p.status, kErrMmaWaitFull)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t sa = smem_u32(ring + stage * kGpStageBytes), sb = sa + kGpHalf;
 #pragma unroll
-          for (int kk = 0; kk < kGpBK / 16; ++kk)
-            gp_mma(tmem + acc * 256, umma_desc_k_sw128(sa + kk * 32), umma_desc_k_sw128(sb + kk * 32), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-          gp_commit(&empty_bar[stage]);
-          if (++stage == kGpStages) stage = 0, phase ^= 1u;
+            for (int kk = 0; kk < kGpBK / 16; ++kk)
+              gp_mma(tmem + acc * 256, umma_desc_k_sw128(sa + kk * 32), umma_desc_k_sw128(sb + kk * 32), idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+            gp_commit(&empty_bar[stage]);
+            if (++stage == kGpStages) stage = 0, phase ^= 1u;
+          }
+          if (!ok) break;
+          gp_commit(&tmem_full[acc]);
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1u;
         }
-        if (!ok) break;
-        gp_commit(&tmem_full[acc]);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
       }
     }
     __syncwarp();
   } else {
-    const int q = warp & 3, row = q * 32 + lane;
+    const int q = warp & 3, row = q * 32 + lane, col0 = (warp - 2) / 4 * kHlCols;
     const uint32_t done = gp_leader(tmem_empty);
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = pair; t < tiles; t += pairs) {
+    bool all = true;
+    for (int t = pair; all && t < tiles; t += pairs) {
       int m0, f0;
       place(t, m0, f0);
-      const int m = m0 + rank * 128 + row, valid = min(256, p.V - f0);
+      f0 += col0;
+      const int m = m0 + rank * 128 + row, valid = p.V - f0;            // (below 1 where the vocabulary ends in the first half)
       const bool live = m < p.M;
       const long long own_col = live ? head_id(p, m) - f0 : -1;
-      const bool ok = gp_wait(&tmem_full[acc], acc_phase, p.status, kErrEpilogueWait);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after_sync();
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-      LpSums a{-INFINITY, 0.f, 0.f};
-      float own = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < valid; c += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32(taddr + c, r);
-        tmem_ld_wait();
-        float z[32], top = -INFINITY;
+      float z[kHlCols];
+      for (int kb0 = 0; kb0 < num_kb; kb0 += kHlSegment) {
+        const bool ok = gp_wait(&tmem_full[acc], acc_phase, p.status, kErrEpilogueWait);
+        all = __all_sync(0xffffffffu, ok);
+        if (!all) break;
+        tc_fence_after_sync();
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * 256 + col0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          z[i] = __uint_as_float(r[i]);
-          if constexpr (SHAPED) z[i] = lp_transform(z[i], min(f0 + c + i, p.V - 1), p.bias, p.bias_fp32, p.scale, p.softcap);
+        for (int c = 0; c < kHlCols; c += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c, r);
+          tmem_ld_wait();
+          if (kb0 == 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[c + i] = __uint_as_float(r[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[c + i] += __uint_as_float(r[i]);
+          }
         }
-        if (c + 32 > valid) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i >= valid) z[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, z[i]);            // (NaN is dropped here and by the floor below: it counts as -inf)
-        if (top > a.m) a = lp_rescale(a, top);
-        if (lp_plain(a.m)) {
-          const float low = lp_floor(a.m);
-          lp_pair s2 = lp_two(a.s, 0.f), t2 = lp_two(a.t, 0.f);
-          float f[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = fmaxf(z[i], low);
-          lp_add(f, lp_two(-a.m, -a.m), s2, t2);
-          const float2 s = lp_both(s2), t = lp_both(t2);
-          a.s = s.x + s.y;
-          a.t = t.x + t.y;
-        } else if (a.m != -INFINITY) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) a.s += z[i] == a.m ? 1.f : 0.f;
-        }
-        if (own_col >= c && own_col < c + 32) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (own_col == c + i) own = z[i] != z[i] ? -INFINITY : z[i];
-        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) gp_arrive(done + 8 * acc);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) gp_arrive(done + 8 * acc);
+      if (!all) break;
+      if constexpr (SHAPED) {
+#pragma unroll
+        for (int i = 0; i < kHlCols; ++i) z[i] = lp_transform(z[i], min(f0 + i, p.V - 1), p.bias, p.bias_fp32, p.scale, p.softcap);
+      }
+      if (valid < kHlCols) {
+#pragma unroll
+        for (int i = 0; i < kHlCols; ++i)
+          if (i >= valid) z[i] = -INFINITY;
+      }
+      if (own_col >= 0 && own_col < min(valid, kHlCols)) {
+        float own = 0.f;
+#pragma unroll
+        for (int i = 0; i < kHlCols; ++i)
+          if (own_col == i) own = z[i] != z[i] ? -INFINITY : z[i];
+        p.partials[static_cast<size_t>(p.tiles_n) * 6 * p.M + m] = own;
+      }
+      LpSums a{-INFINITY, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kHlCols; ++i) a.m = fmaxf(a.m, z[i]);          // (NaN is dropped here and by the floor below: it counts as -inf)
+      if (lp_plain(a.m)) {
+        const float low = lp_floor(a.m);
+        lp_pair s2 = lp_two(0.f, 0.f), t2 = s2;
+#pragma unroll
+        for (int i = 0; i < kHlCols; ++i) z[i] = fmaxf(z[i], low);
+        lp_add(z, lp_two(-a.m, -a.m), s2, t2);
+        const float2 s = lp_both(s2), t = lp_both(t2);
+        a.s = s.x + s.y;
+        a.t = t.x + t.y;
+      } else if (a.m != -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < kHlCols; ++i) a.s += z[i] == a.m ? 1.f : 0.f;
+      }
       if (live) {
-        float* out = p.partials + static_cast<size_t>(f0 / 256) * 3 * p.M + m;
+        float* out = p.partials + static_cast<size_t>(f0 / kHlCols) * 3 * p.M + m;
         out[0] = a.m;
         out[p.M] = a.s;
         out[2 * static_cast<size_t>(p.M)] = a.t;
-        if (own_col >= 0 && own_col < valid) p.partials[static_cast<size_t>(p.tiles_n) * 3 * p.M + m] = own;
       }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
     }
   }
 
@@ -219,7 +242,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   }
 }
 
-// Joins the column tiles of 32 rows (a lane each), a warp every 32nd tile, in a fixed order.
+// Joins the halves of the column tiles of 32 rows (a lane each), a warp every 32nd tile, in a fixed order.
 __global__ void __launch_bounds__(1024) head_join_kernel(const HeadParams p) {
   __shared__ float part[3][32][33];
   pdl_trigger();
@@ -228,7 +251,7 @@ __global__ void __launch_bounds__(1024) head_join_kernel(const HeadParams p) {
   LpSums a{-INFINITY, 0.f, 0.f};
   if (m < p.M) {
 #pragma unroll 4
-    for (int t = warp; t < p.tiles_n; t += 32) {
+    for (int t = warp; t < 2 * p.tiles_n; t += 32) {
       const float* src = p.partials + static_cast<size_t>(t) * 3 * p.M + m;
       a = lp_join(a, {src[0], src[p.M], src[2 * static_cast<size_t>(p.M)]});
     }
@@ -240,7 +263,7 @@ __global__ void __launch_bounds__(1024) head_join_kernel(const HeadParams p) {
   const long long id = head_id(p, m);
   p.lse[m] = lp_lse(a);
   p.entropy[m] = lp_entropy(a);
-  p.logprob[m] = id < 0 || id >= p.V ? __int_as_float(0x7fc00000) : lp_log(p.partials[static_cast<size_t>(p.tiles_n) * 3 * p.M + m], a);
+  p.logprob[m] = id < 0 || id >= p.V ? __int_as_float(0x7fc00000) : lp_log(p.partials[static_cast<size_t>(p.tiles_n) * 6 * p.M + m], a);
 }
 
 }  // namespace mx
@@ -264,7 +287,7 @@ extern "C" int mx_head_logprobs(const void* x, const void* w, const void* ids, i
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n, most = device_sm_count() / 2;
   if (tiles > 0x7fffffffll) return -1;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  e = launch_kernel(kern, dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most)), dim3(kGpThreads), kGpSmem, stream, map_x, map_w, p);
+  e = launch_kernel(kern, dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most)), dim3(kHlThreads), kGpSmem, stream, map_x, map_w, p);
   if (e != cudaSuccess) return static_cast<int>(e);
   return static_cast<int>(launch_kernel(head_join_kernel, dim3((M + 31) / 32), dim3(1024), 0, stream, p));
 }

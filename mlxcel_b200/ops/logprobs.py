@@ -90,8 +90,8 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: 
     ldx, ldw = x.stride(0) if R > 1 else K, w.stride(0) if V > 1 else K
     if R and (R > FEW_ROWS or V * K <= LARGE_WEIGHTS) and x.dtype == torch.bfloat16 and not (K % 8 or ldx % 8 or ldw % 8 or (x.data_ptr() | w.data_ptr()) % 16):
         tiles, ids = -(-V // 256), ids.contiguous()
-        part = min(R, max(256, PARTIAL_BYTES // (12 * tiles) // 256 * 256))
-        partials = torch.empty((3 * tiles + 1) * part, **f)
+        part = min(R, max(256, PARTIAL_BYTES // (24 * tiles) // 256 * 256))
+        partials = torch.empty((6 * tiles + 1) * part, **f)
         for r0 in range(0, R, part):
             _lib.launch_on(x.device, "mx_head_logprobs", x.data_ptr() + 2 * r0 * ldx, w.data_ptr(), ids.data_ptr() + r0 * ids.element_size(),
                            int(ids.dtype == torch.int64), _lib.ptr(bias), int(bias is not None and bias.dtype == torch.float32), float(scale),
