@@ -7,9 +7,9 @@
 // Logits of 2047 rows over 128256 tokens would be 1 GB of fp32; what is written instead is 12 MB. The logits are never rounded.
 //
 // Bound by the tensor cores under the power cap: a tile's products take 8 K cycles an SM, its epilogue about 3000 beside them, whose
-// instructions cost power and with it clock. Measured, in a row (us): 2047 rows, K 4096, V 128256 1870 (1.15 PFLOP/s); 1790 with the sums
-// left in the tensor core over all of K (3e-6 from the 64-bit result in place of 7e-7), 1910 with the changes of SHAPED made in any
-// case; the same product by gemm_pair.cu, which writes 525 MB of bf16 logits, 1750, by cuBLAS 1550.
+// instructions cost power and with it clock. Measured, in a row (us): 2047 rows, K 4096, V 128256 1870 (1.15 PFLOP/s); the same product
+// by gemm_pair.cu, which writes 525 MB of bf16 logits, 1750, by cuBLAS 1550. With the sums left in the tensor core over all of K 1790,
+// and 3e-6 from the 64-bit result in place of 7e-7; with the changes of SHAPED made in any case 120 more.
 #include <cooperative_groups.h>
 
 #include "api.h"

@@ -12,8 +12,8 @@ from . import _lib, linear, reference as ref
 MAX_TOP = 64
 _ARGS = struct.Struct("PqPPPPPPPiiiiiiiff")        # MxTokenLogprobs of csrc/api.h
 # head_logprobs keeps its logits on the chip, unless few rows meet large weights: there both forms read the weights at the pace of the
-# memory, and the smaller tiles of `linear` are the faster ones. us on the chip / through memory: 8 rows, 128256 x 4096 217 / 171, 64
-# rows 210 / 191, 100 rows 215 / 222, 256 rows 244 / 480; 8 rows, 50257 x 1024 49 / 61, 5000 x 512 27 / 59.
+# memory, and the smaller tiles of `linear` are the faster ones. us on the chip / through memory: 8 rows, 128256 x 4096 230 / 174, 64
+# rows 226 / 194, 100 rows 231 / 229, 256 rows 251 / 437; 8 rows, 50257 x 1024 50 / 70, 5000 x 512 27 / 58.
 FEW_ROWS, LARGE_WEIGHTS = 64, 1 << 28
 PARTIAL_BYTES = 256 << 20        # of the column tiles' sums that are held at once
 
