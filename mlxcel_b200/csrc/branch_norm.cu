@@ -81,6 +81,54 @@ struct Pack {
   }
 };
 
+// a = a b + c (b and c as many or one number), a = a b, and a^2 added to s; rows of bf16, which take more instructions per byte, two
+// elements at a time.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+template <int V>
+__device__ __forceinline__ void mul_add(float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; j += V == 8 ? 2 : 1) {
+    if constexpr (V == 8) {
+      const float2 r = __ffma2_rn(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]), make_float2(c[j], c[j + 1]));
+      a[j] = r.x, a[j + 1] = r.y;
+    } else {
+      a[j] = fmaf(a[j], b[j], c[j]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_add(float (&a)[V], float b, float c) {
+#pragma unroll
+  for (int j = 0; j < V; j += V == 8 ? 2 : 1) {
+    if constexpr (V == 8) {
+      const float2 r = __ffma2_rn(make_float2(a[j], a[j + 1]), both(b), both(c));
+      a[j] = r.x, a[j + 1] = r.y;
+    } else {
+      a[j] = fmaf(a[j], b, c);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul(float (&a)[V], const float (&b)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; j += V == 8 ? 2 : 1) {
+    if constexpr (V == 8) {
+      const float2 r = __fmul2_rn(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]));
+      a[j] = r.x, a[j + 1] = r.y;
+    } else {
+      a[j] *= b[j];
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_squares(float2& s, const float (&a)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; j += V == 8 ? 2 : 1) {
+    if constexpr (V == 8) s = __ffma2_rn(make_float2(a[j], a[j + 1]), make_float2(a[j], a[j + 1]), s);
+    else s.x = fmaf(a[j], a[j], s.x);
+  }
+}
+
 // Rows that do not start on 16 bytes but all at the same place within 16 bytes (rows of an odd length behind each other) are covered by
 // the aligned vectors that hold them: vector v has the elements v V - o ... of a row that starts o elements behind a boundary. Ends are
 // read and written element by element (what is beyond the row counts as 0 and is not touched).
@@ -143,7 +191,7 @@ __device__ __forceinline__ void load_shifted(Pack<T, V>& d, const T* w, int v, i
 }
 
 template <typename T, int V, int VPT, int MOST, bool LAYER, bool SHIFT>
-__global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParams p) {
+__global__ void __launch_bounds__(MOST, VPT > 4 ? 1 : MOST == 256 ? 3 : MOST == 512 ? 2 : 1) branch_norm_kernel(const BranchNormParams p) {
   __shared__ float red[3][32];
   pdl_trigger();
   pdl_wait();
@@ -181,48 +229,53 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
   }
   float rstd = 1.f;
   if (post) {
-    float ss = 0.f;
+    float2 ss = both(0.f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (threadIdx.x + i * blockDim.x < nvec) {
         float f[V];
         xv[i].widen(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) ss += f[j] * f[j];
+        add_squares(ss, f);
       }
     }
-    rstd = rsqrtf(row_sum(ss, red[0]) / static_cast<float>(p.dim) + p.eps);
+    rstd = rsqrtf(row_sum(ss.x + ss.y, red[0]) / static_cast<float>(p.dim) + p.eps);
   }
-  float hv[VPT][V], stat = 0.f;
+  float hv[VPT][V];
+  float2 stat2 = both(0.f);
+  const float factor = rstd * p.scale;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v < nvec) {
-      xv[i].widen(hv[i]);
       Pack<T, V> t;
-      float f[V];
-      if (post) {
+      float f[V], g[V];
+      if (post) {                                            // what the branch is multiplied by
         wv[i].widen(f);
+        mul_add(f, factor, factor * p.w_bias);
+      } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) hv[i][j] *= rstd * (f[j] + p.w_bias);
+        for (int j = 0; j < V; ++j) f[j] = factor;
       }
       if (gate) {
         weights(t, gate, v);
-        t.widen(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) hv[i][j] *= f[j];
+        t.widen(g);
+        mul(f, g);
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) hv[i][j] *= p.scale;
+      xv[i].widen(hv[i]);
       if (res) {
-        rv[i].widen(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) hv[i][j] += f[j];
+        rv[i].widen(g);
+        mul_add(hv[i], f, g);
+      } else {
+        mul(hv[i], f);
       }
       t.narrow(hv[i]);
       put(t, static_cast<T*>(p.h) + row * p.ldh, v);
+      if constexpr (LAYER) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) stat += LAYER ? hv[i][j] : hv[i][j] * hv[i][j];
+        for (int j = 0; j < V; ++j) stat2.x += hv[i][j];
+      } else {
+        add_squares(stat2, hv[i]);
+      }
     }
   }
   if (pre == nullptr) return;
@@ -232,7 +285,7 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
     if (v < nvec) weights(wv[i], pre, v);
   }
   float mean = 0.f;
-  stat = row_sum(stat, red[1]) / static_cast<float>(p.dim);
+  float stat = row_sum(stat2.x + stat2.y, red[1]) / static_cast<float>(p.dim);
   if constexpr (LAYER) {                    // the variance from the centred row: no cancellation where the mean is large
     mean = stat;
     float ss = 0.f;
@@ -257,13 +310,18 @@ __global__ void __launch_bounds__(MOST) branch_norm_kernel(const BranchNormParam
       Pack<T, V> t;
       float f[V];
       wv[i].widen(f);
+      mul_add(f, rstd, rstd * p.w_bias);
+      if constexpr (LAYER) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) hv[i][j] = (hv[i][j] - mean) * rstd * (f[j] + p.w_bias);
+        for (int j = 0; j < V; ++j) hv[i][j] -= mean;
+      }
       if (bias) {
+        float g[V];
         weights(t, bias, v);
-        t.widen(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) hv[i][j] += f[j];
+        t.widen(g);
+        mul_add(hv[i], f, g);
+      } else {
+        mul(hv[i], f);
       }
       t.narrow(hv[i]);
       put(t, static_cast<T*>(p.y) + row * p.ldy, v);
@@ -284,11 +342,16 @@ static int launch_branch_norm(const BranchNormParams& p, int rows, cudaStream_t 
   if (threads > 1024) return -1;                            // (a shifted row of the greatest length: left to the form by elements)
   auto run = [&](auto kern) { return static_cast<int>(launch_kernel(kern, dim3(rows), dim3(threads), 0, stream, p)); };
   if (each == 1) return run(branch_norm_kernel<T, V, 1, 1024, LAYER, SHIFT>);
-  if (each == 2) return threads <= 256 ? run(branch_norm_kernel<T, V, 2, 256, LAYER, SHIFT>) : run(branch_norm_kernel<T, V, 2, 1024, LAYER, SHIFT>);
-  if (each == 4) return threads <= 256 ? run(branch_norm_kernel<T, V, 4, 256, LAYER, SHIFT>) : run(branch_norm_kernel<T, V, 4, 1024, LAYER, SHIFT>);
+#define MX_BRANCH(VPT_)                                                                  \
+  if (threads <= 256) return run(branch_norm_kernel<T, V, VPT_, 256, LAYER, SHIFT>);     \
+  if (threads <= 512) return run(branch_norm_kernel<T, V, VPT_, 512, LAYER, SHIFT>);     \
+  return run(branch_norm_kernel<T, V, VPT_, 1024, LAYER, SHIFT>)
+  if (each == 2) { MX_BRANCH(2); }
+  if (each == 4) { MX_BRANCH(4); }
   if constexpr (V < 8) {
-    if (each == 8) return threads <= 256 ? run(branch_norm_kernel<T, V, 8, 256, LAYER, SHIFT>) : run(branch_norm_kernel<T, V, 8, 1024, LAYER, SHIFT>);
+    if (each == 8) { MX_BRANCH(8); }
   }
+#undef MX_BRANCH
   if constexpr (V == 1) {
     if (each == 16) return run(branch_norm_kernel<T, V, 16, 1024, LAYER, SHIFT>);
     return run(branch_norm_kernel<T, V, 32, 1024, LAYER, SHIFT>);
