@@ -8,9 +8,10 @@
 // of the rounded row: what a later reader of the stream would compute. b and the scaled branch are not rounded in between.
 //
 // Bound by memory: x and residual in, h and y out, four rows. The row stays in registers between its reductions (two for rms, three
-// with the mean of a layer norm). Measured (us, of what a copy of these bytes would take): 8192 x 5120 bf16 64 (79 %; 83 with one
-// access per thread and the weights asked for when they are needed), 8192 x 4096 47 (88 %), 2000 x 8192 fp32 45 (89 %), one row of 2560
-// 2.2; rows of an odd length: 8192 x 5119 143 (241 element by element), 8192 x 1003 26 (32).
+// with the mean of a layer norm). Measured (us, of what a copy of these bytes would take): 8192 x 5120 bf16 62 (82 %; 64 with one
+// element per instruction, 83 with one access per thread and the weights asked for when they are needed, 70 with CTAs that stay and
+// have their next row on its way to shared memory: fewer rows are then between their sums at a time), 8192 x 4096 45 (91 %), 2000 x 8192
+// fp32 45 (89 %), one row of 2560 2.1; rows of an odd length: 8192 x 5119 136 (241 element by element), 8192 x 1003 26 (32).
 #include "api.h"
 #include "common.cuh"
 #include "typed.cuh"
@@ -190,6 +191,7 @@ __device__ __forceinline__ void load_shifted(Pack<T, V>& d, const T* w, int v, i
   }
 }
 
+// (registers: 4 CTAs of 256 threads or 64 a thread cost more in spills than they hide: 8192 x 4096 48 us in place of 45)
 template <typename T, int V, int VPT, int MOST, bool LAYER, bool SHIFT>
 __global__ void __launch_bounds__(MOST, VPT > 4 ? 1 : MOST == 256 ? 3 : MOST == 512 ? 2 : 1) branch_norm_kernel(const BranchNormParams p) {
   __shared__ float red[3][32];
