@@ -55,8 +55,8 @@ def sequence_scores(model, cfg, ids: list[int], block_size: int = 16, row_chunk:
     h = prefill_hidden(model, cfg, ids, block_size)
     tgt = torch.tensor(ids[1:], dtype=torch.long, device=dev)
     own = getattr(model, "token_logprobs", None)
-    if own is not None and not top:
-        row_chunk = max(row_chunk, 8192)                     # (no logits are held for these rows, or few)
+    if not top and h.is_cuda and getattr(model, "scores_from_hidden", False):
+        row_chunk = max(row_chunk, 8192)                     # (no logits are held for these rows)
     parts = []
     for r0 in range(0, T - 1, row_chunk):
         rows = torch.arange(r0, min(r0 + row_chunk, T - 1), device=dev)

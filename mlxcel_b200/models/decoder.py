@@ -620,11 +620,16 @@ class DecoderModel:
             lg = (torch.tanh(lg.float() / c) * c).to(lg.dtype)
         return lg
 
+    @property
+    def scores_from_hidden(self) -> bool:
+        """Whether :meth:`token_logprobs` goes from hidden rows to log probabilities (else through logits)."""
+        return self.comm.tp_size == 1 and not isinstance(self.w.lm_head, QuantizedTensor) and type(self).logits is DecoderModel.logits
+
     def token_logprobs(self, h: torch.Tensor, rows: torch.Tensor | None, ids: torch.Tensor, top: int = 0):
         """:class:`~mlxcel_b200.ops.logprobs.TokenLogprobs` of tokens ``ids`` behind the selected rows. Without alternatives, on one GPU
         and with dense head weights the logits stay on the chip (and are not rounded)."""
         cfg, w = self.cfg, self.w
-        if top or self.comm.tp_size != 1 or isinstance(w.lm_head, QuantizedTensor) or type(self).logits is not DecoderModel.logits:
+        if top or not self.scores_from_hidden:
             return lops.token_logprobs(self.logits(h, rows), ids, top)
         if rows is not None:
             h = h.index_select(0, rows)

@@ -203,3 +203,23 @@ def test_server_returns_alternatives():
             assert "top_logprobs" not in e
     finally:
         worker.shutdown()
+
+
+@pytest.mark.parametrize("through_logits", [False, True])
+def test_scores_hold_few_rows_of_logits(through_logits):
+    """Logits of a long text are never held for more rows than asked for, with a head that scores hidden rows and with one that cannot."""
+    cfg, model = _model()
+    if through_logits:
+        class Wrapped(DecoderModel):
+            def logits(self, h, rows):
+                return super().logits(h, rows)
+        model = Wrapped(cfg, model.w)
+    assert model.scores_from_hidden is not through_logits
+    ids = [(7 * i) % cfg.vocab_size for i in range(90)]
+    want = sequence_scores(model, cfg, ids, 8, row_chunk=89)
+    rows, own = [], model.token_logprobs
+    model.token_logprobs = lambda h, r, i, top=0: (rows.append(r.numel()), own(h, r, i, top))[1]
+    got = sequence_scores(model, cfg, ids, 8, row_chunk=32)
+    assert rows == [32, 32, 25]
+    # the same sums of the same numbers, in products of 32 rows and of 89: fp32 rounding of 64 additions each
+    torch.testing.assert_close(got.logprob, want.logprob, rtol=0, atol=1e-4)
