@@ -569,6 +569,15 @@ def test_head_logprobs_in_parts_and_single_rows(monkeypatch):
     assert not r.logprob.any() and not r.entropy.any()
 
 
+@pytest.mark.parametrize("K", [128, 131])
+def test_head_logprobs_single_row_of_any_stride_through_logits(K, monkeypatch):
+    monkeypatch.setattr(logprobs, "LARGE_WEIGHTS", 0)
+    x, w = _rn(2, K, seed=1), _rn(900, K, seed=2, scale=0.2)
+    ids = torch.tensor([17], device=DEV)
+    for stride in (0, 1, K - 3, K + 5):
+        _check_head(x[0].as_strided((1, K), (stride, 1)), w, ids)
+
+
 def test_head_logprobs_masked_by_bias_and_bad_rows():
     R, V, K = 400, 2000, 128
     x, w = _rn(R, K, seed=1), _rn(V, K, seed=2, scale=0.2)
