@@ -491,6 +491,7 @@ extern "C" int mx_mrope_append(const MxMropeAppend* a, void* stream_) {
   const int T = a->T, D = a->D, rot_dim = a->rot_dim, kv_bits = a->kv_bits;
   if (T <= 0) return 0;
   if (D <= 0 || D > kMropeMaxDim || rot_dim < 0 || rot_dim > D || rot_dim % 2 || a->Hq < 0 || a->Hkv < 0 || a->axes < 1 || a->block_size < 1) return -1;
+  if (a->Hq + a->Hkv == 0) return -1;                        // (threads walk from head to head: without any they would not come to an end)
   if ((kv_bits != 16 && kv_bits != 8 && kv_bits != 4) || (kv_bits != 16 && (D % 64 || a->k_meta == nullptr || a->v_meta == nullptr))) return -1;
   MropeParams p{};
   p.qkv = static_cast<const __nv_bfloat16*>(a->qkv);

@@ -43,6 +43,8 @@ def mrope_append(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch
     ``mscale``. ``q_norm_w`` / ``k_norm_w`` [D]: rms norm of each head before it turns. Values are rounded once, at the end.
     ``out``: where q goes; q's own columns of ``qkv`` are fine, other overlap is not. No two rows may name one slot. A row's axis number
     outside ``positions`` takes the nearest axis."""
+    if D < 1 or Hq < 0 or Hkv < 0 or Hq + Hkv == 0:
+        raise ValueError(f"{Hq} + {Hkv} heads of {D} are no projection")
     T, width = qkv.shape[0], (Hq + 2 * Hkv) * D
     if qkv.dim() != 2 or qkv.shape[1] != width:
         raise ValueError(f"qkv has to be [T, {width}], not {tuple(qkv.shape)}")
