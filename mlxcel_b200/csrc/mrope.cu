@@ -546,9 +546,9 @@ extern "C" int mx_axial_rope(const void* qkv, long long ldqkv, float* q, float* 
   if (D <= 0 || D > kMropeMaxDim || D % 2 || axes < 1) return -1;
   AxialParams p{static_cast<const __nv_bfloat16*>(qkv), q, k, v, {positions, axis, inv_freq, ldp, axes, D / 2}, ldqkv, R, H, D};
   // (16-byte accesses: 33 us where 8-byte ones take 26 with as much in flight, 5476 patches of 16 heads of 80)
-  const int w = mrope_width(4, D, D, reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v),
-                            ldqkv);
-  if (w != 0) {
+  const int w = mrope_width(4, D, D, reinterpret_cast<uintptr_t>(qkv), ldqkv);
+  // (results are written 16 bytes at a time)
+  if (w != 0 && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(v, 16)) {
     const int per = mrope_tokens(R), blocks = (R + per - 1) / per;
     return static_cast<int>(launch_kernel(axial_rope_vec_kernel<4>, dim3(blocks), dim3(kMropeThreads), 0, static_cast<cudaStream_t>(stream_), p, per));
   }
