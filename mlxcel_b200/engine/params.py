@@ -97,4 +97,4 @@ class SamplingParams:
         temperature draw go through the fused CUDA sampler; the rest take the extended chain."""
         return (self.xtc_probability <= 0.0 and
                 self.mirostat == 0 and self.dynatemp_range <= 0.0 and self.dry_multiplier <= 0.0 and
-                not self.logit_bias and self.top_logprobs == 0)
+                not self.logit_bias)

@@ -5,8 +5,8 @@ src/lib/mlxcel-core/src/generate.rs:1296-1340): token bias and penalties → top
 evaluated on the untempered distribution → one temperature scale applied only to the final draw.
 Rows whose parameters are expressible by the fused kernel (top-k, top-p, min-p, top-n-sigma,
 typical-p, temperature) go through ``ops.sample`` in one launch (``fused_eligible``); the rest
-(XTC, mirostat, dynamic temperature, DRY, top-logprobs) take the extended chain below, row by
-row, on device tensors.
+(XTC, mirostat, dynamic temperature, DRY, logit bias) take the extended chain below, row by
+row, on device tensors. Alternatives (``top_logprobs``) are looked up behind either and change no draw.
 """
 from __future__ import annotations
 

@@ -1,10 +1,15 @@
 """Calls at the edge of what the branch norms, the rotary positions with several axes, the moves of pages and the log probabilities
 take, and the paths of models, pool, engine and server around them (CPU)."""
+import copy
 import struct
 
 import pytest
 import torch
 
+from mlxcel_b200.config import preset
+from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
+from mlxcel_b200.models.decoder import DecoderModel
+from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.ops import KVLayer, _lib, rotary
 
 
@@ -23,3 +28,29 @@ def test_mrope_entry_refuses_no_heads_before_it_launches():
     """The C entry checks this itself (it returns before it asks for a device)."""
     args = rotary._ARGS.pack(*([16, 0] * 3), 16, 16, 64, *[16] * 5, 0, 0, 3, 5, 0, 0, 64, 64, 16, 0, 16, 1e-6, 1.0)
     assert len(args) == struct.calcsize(rotary._ARGS.format) and _lib.load().mx_mrope_append(args, None) == -1
+
+
+# ----------------------------------------------------------------------------- log probabilities of requests
+def _tiny(seed=0, dtype=torch.float32):
+    cfg = copy.deepcopy(preset("tiny-qwen3"))
+    return cfg, DecoderModel(cfg, random_weights(cfg, seed=seed, dtype=dtype, std=0.08))
+
+
+def test_alternatives_change_no_draw():
+    """Seeded requests, alone and beside others, draw the same tokens whether or not they ask for alternatives."""
+    cfg, model = _tiny()
+    base = [dict(temperature=0.9, top_p=0.9, seed=3), dict(temperature=1.3, top_k=50, seed=4), dict(temperature=0.7, min_p=0.05, typical_p=0.9, seed=5),
+            dict(temperature=0.0)]
+
+    def run(extra):
+        eng = Engine(model, cfg, EngineConfig(max_batch=4, max_num_batched_tokens=64, num_blocks=32, max_model_len=128, cuda_graphs=False))
+        sids = [eng.add_request([1, 2, 3, 4 + i], SamplingParams(max_tokens=8, ignore_eos=True, **b, **e)) for i, (b, e) in enumerate(zip(base, extra))]
+        while eng.has_work():
+            eng.step()
+        return [eng.seqs[s] for s in sids]
+    want = run([{}] * 4)
+    for extra in ([dict(logprobs=True, top_logprobs=5)] * 4, [dict(logprobs=True, top_logprobs=1 + 3 * i) if i % 2 else {} for i in range(4)],
+                  [dict(top_logprobs=4)] * 4):
+        for s, w, e in zip(run(extra), want, extra):
+            assert s.output == w.output, e
+            assert [len(lp.top) for lp in s.logprobs] == ([e["top_logprobs"]] * 8 if e.get("logprobs") else [])
