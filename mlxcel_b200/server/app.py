@@ -485,6 +485,9 @@ def create_app(state: ServerState) -> FastAPI:
     @app.post("/v1/completions")
     async def completions(body: dict):
         sp = sampling_from_body(body, 16)
+        many = body.get("logprobs")
+        if not sp.top_logprobs and isinstance(many, int) and not isinstance(many, bool):
+            sp.top_logprobs = max(0, many)                   # a number of alternatives asks for them as ``top_logprobs`` does
         ids = _prompt_ids(body.get("prompt", ""))
         cid, created = "cmpl-" + uuid.uuid4().hex[:24], int(time.time())
         try:
@@ -513,13 +516,12 @@ def create_app(state: ServerState) -> FastAPI:
             from ..engine.scoring import sequence_scores
             from ..ops.logprobs import MAX_TOP
             eng = state.worker.engine
-            # alternatives at every place of the prompt: ``top_logprobs``, or the count that ``logprobs`` gives
-            many = body.get("logprobs")
-            many = many if isinstance(many, int) and not isinstance(many, bool) else 0
-            many = min(max(0, sp.top_logprobs or many), MAX_TOP, eng.cfg.vocab_size)
-            scores = await asyncio.get_running_loop().run_in_executor(
-                None, lambda: sequence_scores(eng.model, eng.cfg, ids, eng.ecfg.block_size, top=many))
-            plp = scores.logprob.tolist()
+            many = min(max(0, sp.top_logprobs), MAX_TOP, eng.cfg.vocab_size)       # alternatives at every place
+
+            def score():
+                r = sequence_scores(eng.model, eng.cfg, ids, eng.ecfg.block_size, top=many)
+                return r.logprob.tolist(), [_ranked(zip(i, v)) for i, v in zip(r.top_ids.tolist(), r.top_logprobs.tolist())] if many else []
+            plp, ptop = await asyncio.get_running_loop().run_in_executor(None, score)
             ptoks = [tk.decode([t], skip_special_tokens=False) for t in ids]
             offs, pos = [], 0
             for piece in ptoks:
@@ -538,8 +540,8 @@ def create_app(state: ServerState) -> FastAPI:
                                    "token_logprobs": [None] + plp + (gen_lps if sp.logprobs else [None] * len(gen_toks)),
                                    "text_offset": offs}}
             if many:
-                choice["logprobs"]["top_logprobs"] = ([None] + [_ranked(zip(i, v)) for i, v in zip(scores.top_ids.tolist(), scores.top_logprobs.tolist())]
-                                                      + [_ranked(getattr(lp, "top", [])) for lp in gen_lps if sp.logprobs])
+                choice["logprobs"]["top_logprobs"] = [None] + ptop + ([_ranked(getattr(lp, "top", [])) for lp in gen_lps] if sp.logprobs
+                                                                      else [None] * len(gen_toks))
             return {"id": cid, "object": "text_completion", "created": created, "model": state.model_id, "choices": [choice],
                     "usage": usage or {"prompt_tokens": len(ids), "completion_tokens": 0, "total_tokens": len(ids)}}
         try:

@@ -1,16 +1,21 @@
 """Calls at the edge of what the branch norms, the rotary positions with several axes, the moves of pages and the log probabilities
 take, and the paths of models, pool, engine and server around them (CPU)."""
 import copy
+import math
 import struct
 
 import pytest
 import torch
+from fastapi.testclient import TestClient
 
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
 from mlxcel_b200.models.decoder import DecoderModel
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.ops import KVLayer, _lib, rotary
+from mlxcel_b200.server.app import ServerState, create_app
+from mlxcel_b200.server.worker import ModelWorker
+from mlxcel_b200.tokenizer import ByteTokenizer
 
 
 # ----------------------------------------------------------------------------- rotary positions
@@ -54,3 +59,46 @@ def test_alternatives_change_no_draw():
         for s, w, e in zip(run(extra), want, extra):
             assert s.output == w.output, e
             assert [len(lp.top) for lp in s.logprobs] == ([e["top_logprobs"]] * 8 if e.get("logprobs") else [])
+
+
+@pytest.fixture(scope="module")
+def client():
+    cfg = preset("tiny-llama")
+    eng = Engine(DecoderModel(cfg, random_weights(cfg, seed=0, dtype=torch.float32, std=0.05)), cfg,
+                 EngineConfig(max_batch=4, max_num_batched_tokens=256, num_blocks=128, max_model_len=512, cuda_graphs=False))
+    tk = ByteTokenizer(cfg.vocab_size)
+    worker = ModelWorker(eng, tk, "tiny")
+    try:
+        with TestClient(create_app(ServerState(worker, tk, "tiny"))) as c:
+            yield c
+    finally:
+        worker.shutdown()
+
+
+def _complete(client, **body):
+    r = client.post("/v1/completions", json={"prompt": "hello", "max_tokens": 3, "temperature": 0, "ignore_eos": True, **body})
+    assert r.status_code == 200
+    return r.json()["choices"][0].get("logprobs")
+
+
+@pytest.mark.parametrize("ask", [dict(logprobs=4), dict(logprobs=True, top_logprobs=4), dict(logprobs=2, top_logprobs=4)])
+def test_echo_lists_alternatives_of_prompt_and_generated_tokens_alike(client, ask):
+    e = _complete(client, echo=True, **ask)
+    n = len(e["tokens"])
+    assert len(e["token_logprobs"]) == len(e["top_logprobs"]) == n and e["top_logprobs"][0] is None
+    for lp, top in zip(e["token_logprobs"][1:], e["top_logprobs"][1:]):
+        assert 1 <= len(top) <= 4 and max(top.values()) >= lp - 1e-5
+    for lp, top in zip(e["token_logprobs"][-3:], e["top_logprobs"][-3:]):           # (drawn greedily: the most likely)
+        assert math.isclose(max(top.values()), lp, abs_tol=1e-5)
+
+
+def test_echo_without_log_probabilities_of_generated_tokens(client):
+    e = _complete(client, echo=True, top_logprobs=4)
+    assert len(e["top_logprobs"]) == len(e["token_logprobs"]) == len(e["tokens"])
+    assert e["top_logprobs"][-3:] == e["token_logprobs"][-3:] == [None] * 3 and all(e["top_logprobs"][1:-3])
+
+
+def test_a_number_of_log_probabilities_gives_alternatives_without_echo_too(client):
+    got, want = _complete(client, logprobs=3), _complete(client, logprobs=True, top_logprobs=3)
+    assert got == want and len(got["top_logprobs"]) == 3 and all(got["top_logprobs"])
+    assert "top_logprobs" not in _complete(client, logprobs=True)
