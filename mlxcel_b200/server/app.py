@@ -428,10 +428,11 @@ def create_app(state: ServerState) -> FastAPI:
 
     # ------------------------------------------------------------------ completions
     def _ranked(pairs) -> dict:
-        """{token text: log probability} of (id, log probability) pairs, most likely first."""
+        """{token text: log probability} of (id, log probability) pairs, most likely first, without those of no probability."""
         out: dict = {}
         for t, lp in pairs:
-            out.setdefault(tk.decode([t]), lp)
+            if lp > float("-inf"):                           # (no number of JSON)
+                out.setdefault(tk.decode([t]), lp)
         return out
 
     def _alternatives(lp) -> dict:

@@ -61,18 +61,24 @@ def test_alternatives_change_no_draw():
             assert [len(lp.top) for lp in s.logprobs] == ([e["top_logprobs"]] * 8 if e.get("logprobs") else [])
 
 
-@pytest.fixture(scope="module")
-def client():
+def _serve(allowed=None):
+    """A client of a tiny model, whose head allows all tokens or those of a text."""
     cfg = preset("tiny-llama")
-    eng = Engine(DecoderModel(cfg, random_weights(cfg, seed=0, dtype=torch.float32, std=0.05)), cfg,
-                 EngineConfig(max_batch=4, max_num_batched_tokens=256, num_blocks=128, max_model_len=512, cuda_graphs=False))
-    tk = ByteTokenizer(cfg.vocab_size)
+    w, tk = random_weights(cfg, seed=0, dtype=torch.float32, std=0.05), ByteTokenizer(cfg.vocab_size)
+    if allowed:
+        w.extra["lm_head_b"] = torch.full((cfg.vocab_size,), float("-inf")).index_fill_(0, torch.tensor(tk.encode(allowed)), 0.0)
+    eng = Engine(DecoderModel(cfg, w), cfg, EngineConfig(max_batch=4, max_num_batched_tokens=256, num_blocks=128, max_model_len=512, cuda_graphs=False))
     worker = ModelWorker(eng, tk, "tiny")
     try:
         with TestClient(create_app(ServerState(worker, tk, "tiny"))) as c:
             yield c
     finally:
         worker.shutdown()
+
+
+@pytest.fixture(scope="module")
+def client():
+    yield from _serve()
 
 
 def _complete(client, **body):
@@ -102,3 +108,13 @@ def test_a_number_of_log_probabilities_gives_alternatives_without_echo_too(clien
     got, want = _complete(client, logprobs=3), _complete(client, logprobs=True, top_logprobs=3)
     assert got == want and len(got["top_logprobs"]) == 3 and all(got["top_logprobs"])
     assert "top_logprobs" not in _complete(client, logprobs=True)
+
+
+def test_echo_lists_no_alternatives_without_probability():
+    """Fewer tokens have a probability than alternatives are asked for: the answer stays JSON and lists those."""
+    served = _serve("hello")
+    try:
+        e = _complete(next(served), echo=True, logprobs=20)
+        assert all(set(top) == set("helo") for top in e["top_logprobs"][1:])
+    finally:
+        served.close()
