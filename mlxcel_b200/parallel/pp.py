@@ -17,7 +17,9 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
+from ..engine.sampler import TokenLogprob
 from ..models.decoder import DecoderModel, StepBatch
+from ..ops.logprobs import MAX_TOP
 
 
 class PipelineContext:
@@ -137,24 +139,40 @@ class PipelineModel(DecoderModel):
         return t.cpu().tolist()
 
     def sample_and_share(self, logits, seqs, sampler):
-        """Sample on the last stage and broadcast the token ids (and log-probabilities when a row
+        """Sample on the last stage and broadcast the token ids (and log-probabilities and alternatives when a row
         asks for them) to every rank: R * 4 bytes per step instead of R * vocab logits."""
         ctx = self.ctx
         R = len(seqs)
         want_lp = any(s.params.logprobs for s in seqs)
+        asked = [s.params.logprobs and s.params.top_logprobs > 0 for s in seqs]
+        many = min(max([s.params.top_logprobs for s, a in zip(seqs, asked) if a], default=0), MAX_TOP)
+        top_ids = top_lps = None
         if ctx.is_last:
             toks, lps = sampler.sample(logits, seqs)
             t = torch.tensor(toks, dtype=torch.int32, device=self.device)
             lp = torch.tensor([float(x) if x is not None else 0.0 for x in (lps or [0.0] * R)],
                               dtype=torch.float32, device=self.device) if want_lp else None
+            if many:                                    # rows of (id, log probability), -1 behind the last
+                pairs = [(getattr(x, "top", []) + [(-1, 0.0)] * many)[:many] for x in lps]
+                top_ids = torch.tensor([[i for i, _ in row] for row in pairs], dtype=torch.int32, device=self.device)
+                top_lps = torch.tensor([[v for _, v in row] for row in pairs], dtype=torch.float32, device=self.device)
         else:
             t = torch.empty(R, dtype=torch.int32, device=self.device)
             lp = torch.empty(R, dtype=torch.float32, device=self.device) if want_lp else None
-        dist.broadcast(t, ctx.last_stage_rank0, group=ctx.group)
-        if lp is not None:
-            dist.broadcast(lp, ctx.last_stage_rank0, group=ctx.group)
+            if many:
+                top_ids = torch.empty(R, many, dtype=torch.int32, device=self.device)
+                top_lps = torch.empty(R, many, dtype=torch.float32, device=self.device)
+        for x in (t, lp, top_ids, top_lps):
+            if x is not None:
+                dist.broadcast(x, ctx.last_stage_rank0, group=ctx.group)
         ctx.stats["token_bytes"] = ctx.stats.get("token_bytes", 0) + 4 * R
-        return t.cpu().tolist(), (lp.cpu().tolist() if lp is not None else None)
+        out = lp.cpu().tolist() if lp is not None else None
+        if many:
+            for i, (ids, vals) in enumerate(zip(top_ids.cpu().tolist(), top_lps.cpu().tolist())):
+                if asked[i]:
+                    out[i] = TokenLogprob(out[i])
+                    out[i].top = [(j, v) for j, v in zip(ids, vals) if j >= 0]
+        return t.cpu().tolist(), out
 
 
 class RemoteDrafter:

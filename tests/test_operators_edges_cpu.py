@@ -2,7 +2,12 @@
 take, and the paths of models, pool, engine and server around them (CPU)."""
 import copy
 import math
+import os
+import socket
 import struct
+import subprocess
+import sys
+import textwrap
 
 import pytest
 import torch
@@ -118,3 +123,54 @@ def test_echo_lists_no_alternatives_without_probability():
         assert all(set(top) == set("helo") for top in e["top_logprobs"][1:])
     finally:
         served.close()
+
+
+PIPELINE = """
+import sys, torch, torch.distributed as dist
+sys.path.insert(0, %r)
+dist.init_process_group("gloo")
+rank, world = dist.get_rank(), dist.get_world_size()
+from mlxcel_b200.config import preset
+from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
+from mlxcel_b200.models.decoder import DecoderModel
+from mlxcel_b200.models.weights import random_weights
+from mlxcel_b200.loading.shard import shard_weights, partition_layers
+from mlxcel_b200.parallel.pp import PipelineContext, PipelineModel
+cfg = preset("tiny-qwen3")
+cfg.num_hidden_layers = 4
+full = random_weights(cfg, seed=9, dtype=torch.float32, std=0.05)
+asks = [dict(logprobs=True, top_logprobs=3), {}, dict(logprobs=True), dict(logprobs=True, top_logprobs=100, temperature=0.8, seed=4)]
+def run(model):
+    eng = Engine(model, cfg, EngineConfig(max_batch=4, max_num_batched_tokens=64, num_blocks=64, max_model_len=128, cuda_graphs=False))
+    sids = [eng.add_request([5, 6, 7 + i], SamplingParams(**(dict(max_tokens=4, temperature=0.0, ignore_eos=True) | a))) for i, a in enumerate(asks)]
+    while eng.has_work():
+        eng.step()
+    return [eng.seqs[s] for s in sids]
+want = run(DecoderModel(cfg, full))
+ranges = partition_layers(cfg.num_hidden_layers, world)
+w = shard_weights(cfg, full, 0, 1, layers=ranges[rank], vocab_parallel=False)
+got = run(PipelineModel(cfg, w, PipelineContext(dist.group.WORLD, rank, world), num_micro=2, layer_range=ranges[rank]))
+for g, o, a, count in zip(got, want, asks, (3, None, None, 64)):
+    assert g.output == o.output and len(g.logprobs) == len(o.logprobs) == (4 if a.get("logprobs") else 0), (rank, a)
+    for x, y in zip(g.logprobs, o.logprobs):
+        assert abs(x - y) < 1e-4 and hasattr(x, "top") == hasattr(y, "top") == (count is not None), (rank, a)
+        if count:
+            assert len(x.top) == count and [i for i, _ in x.top][:3] == [i for i, _ in y.top][:3], (rank, a)
+            assert all(abs(u - v) < 1e-4 for (_, u), (_, v) in zip(x.top, y.top)), (rank, a)
+dist.barrier()
+if rank == 0:
+    print("ALTERNATIVES_OK")
+"""
+
+
+def test_alternatives_cross_a_pipeline(tmp_path):
+    """Two stages (gloo): every rank's requests have the alternatives that the last one found."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "pipeline.py"
+    script.write_text(textwrap.dedent(PIPELINE % root))
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1", "--master-port", str(port), str(script)]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=600, env=dict(os.environ, MASTER_ADDR="127.0.0.1", OMP_NUM_THREADS="2"))
+    assert r.returncode == 0 and "ALTERNATIVES_OK" in r.stdout, (r.stdout + r.stderr)[-3000:]
