@@ -485,11 +485,11 @@ class DecoderModel:
             for li, lw in enumerate(w.layers):
                 a = self._attention(li, lw, h, b, kv_layers[li])
                 o = self.comm.row_parallel_linear(a, lw.wo, lw.bo, None)
-                _, h = norms.branch_norm(o, h, post_w=lw.post_attn_norm, eps=eps, w_bias=wb)
+                _, h = norms.branch_step(o, h, post_w=lw.post_attn_norm, eps=eps, w_bias=wb)
                 if cfg.is_moe:
                     raise NotImplementedError("post-norm-only MoE blocks")
                 o = self.comm.row_parallel_linear(self._mlp(lw, h), lw.w_down, lw.b_down, None)
-                _, h = norms.branch_norm(o, h, post_w=lw.post_mlp_norm, eps=eps, w_bias=wb)
+                _, h = norms.branch_step(o, h, post_w=lw.post_mlp_norm, eps=eps, w_bias=wb)
             return h
         # Branches with a norm behind them or a scale end in one kernel: that norm, the scale, the sum, and the norm in front of the
         # next sub-layer (``x``; None where it is still to be taken)
@@ -504,7 +504,7 @@ class DecoderModel:
                 a = (a.float() * torch.sigmoid(_linear_any(x, lw.attn_gate).float())).to(a.dtype)
             if joined:
                 o = self.comm.row_parallel_linear(a, lw.wo, lw.bo, None)
-                x, h = norms.branch_norm(o, h, post_w=lw.post_attn_norm if cfg.post_norms else None, scale=res_mult, pre_w=lw.ln2,
+                x, h = norms.branch_step(o, h, post_w=lw.post_attn_norm if cfg.post_norms else None, scale=res_mult, pre_w=lw.ln2,
                                          eps=eps, w_bias=wb)
             else:
                 h = self.comm.row_parallel_linear(a, lw.wo, lw.bo, h)
@@ -516,7 +516,7 @@ class DecoderModel:
                 else:
                     o = self.comm.row_parallel_linear(self._mlp(lw, x), lw.w_down, lw.b_down, None)
                 nxt = w.layers[li + 1].ln1 if li + 1 < len(w.layers) and b.deepstack is None else None
-                x, h = norms.branch_norm(o, h, post_w=lw.post_mlp_norm if cfg.post_norms else None, scale=res_mult, pre_w=nxt, eps=eps,
+                x, h = norms.branch_step(o, h, post_w=lw.post_mlp_norm if cfg.post_norms else None, scale=res_mult, pre_w=nxt, eps=eps,
                                          w_bias=wb)
             else:
                 if moe:

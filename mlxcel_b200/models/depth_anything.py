@@ -98,7 +98,7 @@ class Dinov2Backbone:
             q, k, v = (qkv[:, :, j].transpose(1, 2) for j in range(3))
             a = F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(N * T, hid).contiguous()
             a = ops.linear(a, b["wo"], bias=b["bo"])
-            y, h = norms.branch_norm(a, h, gate=b["l1"], pre_w=b["n2"][0], pre_b=b["n2"][1], layer_norm=True, eps=self.eps)
+            y, h = norms.branch_step(a, h, gate=b["l1"], pre_w=b["n2"][0], pre_b=b["n2"][1], layer_norm=True, eps=self.eps)
             u = ops.linear(y, b["w1"], bias=b["b1"])
             if self.swiglu:
                 half = u.shape[1] // 2
@@ -107,7 +107,7 @@ class Dinov2Backbone:
                 u = rops.activation(u, "gelu")
             u = ops.linear(u, b["w2"], bias=b["b2"])
             w, b1 = self.blocks[li + 1]["n1"] if li + 1 < len(self.blocks) else (None, None)
-            y, h = norms.branch_norm(u, h, gate=b["l2"], pre_w=w, pre_b=b1, layer_norm=True, eps=self.eps)
+            y, h = norms.branch_step(u, h, gate=b["l2"], pre_w=w, pre_b=b1, layer_norm=True, eps=self.eps)
             emit(li + 1)
         return outs
 

@@ -62,3 +62,12 @@ def branch_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *, post_w
             x.data_ptr(), ldx, at(residual), ldr, at(post_w), at(gate), at(pre_w), at(pre_b), h.data_ptr(), ldh, at(y), dim,
             rows, dim, scale, eps, w_bias, layer_norm, dtype == torch.float32))
     return y, h
+
+
+def branch_step(x: torch.Tensor, residual: torch.Tensor, *, post_w=None, gate=None, scale: float = 1.0, pre_w=None, pre_b=None,
+                layer_norm: bool = False, eps: float = 1e-6, w_bias: float = 0.0) -> tuple[torch.Tensor | None, torch.Tensor]:
+    """:func:`branch_norm` as models take it: on the CPU, where they may hold other types, also for those and for weights of a type of
+    their own (by the plain statement)."""
+    if not x.is_cuda and (x.dtype not in _TYPES or any(t is not None and t.dtype != x.dtype for t in (post_w, gate, pre_w, pre_b))):
+        return ref.branch_norm(x, residual, post_w, gate, scale, pre_w, pre_b, layer_norm, eps, w_bias)
+    return branch_norm(x, residual, post_w=post_w, gate=gate, scale=scale, pre_w=pre_w, pre_b=pre_b, layer_norm=layer_norm, eps=eps, w_bias=w_bias)

@@ -15,7 +15,9 @@ from fastapi.testclient import TestClient
 
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
+from mlxcel_b200.engine.scoring import prefill_hidden
 from mlxcel_b200.models.decoder import DecoderModel
+from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.ops import KVLayer, _lib, rotary
 from mlxcel_b200.server.app import ServerState, create_app
@@ -40,10 +42,61 @@ def test_mrope_entry_refuses_no_heads_before_it_launches():
     assert len(args) == struct.calcsize(rotary._ARGS.format) and _lib.load().mx_mrope_append(args, None) == -1
 
 
-# ----------------------------------------------------------------------------- log probabilities of requests
-def _tiny(seed=0, dtype=torch.float32):
+# ----------------------------------------------------------------------------- models of other types
+NORMS = ("ln1", "ln2", "post_attn_norm", "post_mlp_norm")
+
+
+def _tiny(seed=0, dtype=torch.float32, post_norms=False, norms=None, **extra):
+    """A tiny model whose weights are the same bf16 numbers in any type; ``norms``: the type of its norms around sub-layers."""
     cfg = copy.deepcopy(preset("tiny-qwen3"))
-    return cfg, DecoderModel(cfg, random_weights(cfg, seed=seed, dtype=dtype, std=0.08))
+    cfg.post_norms = post_norms
+    cfg.extra.update(extra)
+    w = random_weights(cfg, seed=seed, dtype=torch.bfloat16, std=0.08)
+    same = w.lm_head is w.embed
+    for lw in w.layers:
+        for n, v in vars(lw).items():
+            if isinstance(v, torch.Tensor):
+                setattr(lw, n, v.to(norms if norms and n in NORMS else dtype))
+    w.embed, w.final_norm = w.embed.to(dtype), w.final_norm.to(dtype)
+    w.lm_head = w.embed if same else w.lm_head.to(dtype)
+    return cfg, DecoderModel(cfg, w)
+
+
+@pytest.mark.parametrize("extra", [dict(post_norms=True), dict(residual_multiplier=0.3)])
+def test_norms_around_sub_layers_in_other_types(extra):
+    """On the CPU models run in any type, and norm weights may be of another than the rows."""
+    ids = [(37 * i) % 1000 for i in range(21)]
+    hidden = lambda **kw: prefill_hidden(*reversed(_tiny(**extra, **kw)), ids, 8)    # noqa: E731
+    want = hidden().double()
+    for dtype, u in ((torch.float16, 2.0 ** -11), (torch.float64, 2.0 ** -24)):
+        got = hidden(dtype=dtype)
+        # 2 layers, each of some 8 roundings to the row type (fp32 within): relative to the spread of the rows
+        assert got.dtype == dtype and (got.double() - want).norm() < 16 * max(u, 2.0 ** -20) * want.norm()
+    assert torch.equal(hidden(dtype=torch.bfloat16), hidden(dtype=torch.bfloat16, norms=torch.float32))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+def test_vision_backbone_in_other_types(dtype):
+    hid, cfg = 32, dict(hidden_size=32, num_hidden_layers=2, num_attention_heads=4, patch_size=4)
+    g = torch.Generator().manual_seed(0)
+    rn = lambda *s, scale=0.2: (torch.randn(*s, generator=g) * scale).to(torch.float16)    # noqa: E731
+    t = {"embeddings.patch_embeddings.projection.weight": rn(hid, 3, 4, 4), "embeddings.patch_embeddings.projection.bias": rn(hid),
+         "embeddings.cls_token": rn(1, 1, hid), "embeddings.position_embeddings": rn(1, 10, hid), "layernorm.weight": 1 + rn(hid), "layernorm.bias": rn(hid)}
+    for i in range(2):
+        p = f"encoder.layer.{i}."
+        for n, shape in (("attention.attention.query", (hid, hid)), ("attention.attention.key", (hid, hid)), ("attention.attention.value", (hid, hid)),
+                         ("attention.output.dense", (hid, hid)), ("mlp.fc1", (64, hid)), ("mlp.fc2", (hid, 64))):
+            t[p + n + ".weight"], t[p + n + ".bias"] = rn(*shape), rn(shape[0])
+        for n in ("norm1", "norm2"):
+            t[p + n + ".weight"], t[p + n + ".bias"] = 1 + rn(hid), rn(hid)
+        t[p + "layer_scale1.lambda1"], t[p + "layer_scale2.lambda1"] = rn(hid), rn(hid)
+    x = rn(2, 3, 12, 12, scale=1.0)
+    want = Dinov2Backbone(cfg, t, dtype=torch.float32).forward(x)[0].double()
+    got = Dinov2Backbone(cfg, t, dtype=dtype).forward(x)[0]
+    assert got.dtype == dtype and (got.double() - want).norm() < 24 * 2.0 ** -11 * want.norm()
+
+
+# ----------------------------------------------------------------------------- log probabilities of requests
 
 
 def test_alternatives_change_no_draw():
@@ -132,7 +185,9 @@ dist.init_process_group("gloo")
 rank, world = dist.get_rank(), dist.get_world_size()
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
+from mlxcel_b200.engine.scoring import prefill_hidden
 from mlxcel_b200.models.decoder import DecoderModel
+from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.loading.shard import shard_weights, partition_layers
 from mlxcel_b200.parallel.pp import PipelineContext, PipelineModel
