@@ -12,7 +12,7 @@ import math
 import torch
 
 from ..models.decoder import StepBatch
-from ..ops.logprobs import TokenLogprobs, token_logprobs
+from ..ops.logprobs import TokenLogprobs, token_logprobs, widened
 
 _SCRATCH_SEQ = -7
 
@@ -61,7 +61,7 @@ def sequence_scores(model, cfg, ids: list[int], block_size: int = 16, row_chunk:
     for r0 in range(0, T - 1, row_chunk):
         rows = torch.arange(r0, min(r0 + row_chunk, T - 1), device=dev)
         want = tgt[r0:r0 + row_chunk]
-        parts.append(own(h, rows, want, top) if own is not None else token_logprobs(model.logits(h, rows), want, top))
+        parts.append(own(h, rows, want, top) if own is not None else token_logprobs(widened(model.logits(h, rows)), want, top))
     return TokenLogprobs(*(torch.cat(p).cpu() for p in zip(*parts)))
 
 

@@ -629,13 +629,14 @@ class DecoderModel:
         """:class:`~mlxcel_b200.ops.logprobs.TokenLogprobs` of tokens ``ids`` behind the selected rows. Without alternatives, on one GPU
         and with dense head weights the logits stay on the chip (and are not rounded)."""
         cfg, w = self.cfg, self.w
-        if top or not self.scores_from_hidden:
-            return lops.token_logprobs(self.logits(h, rows), ids, top)
+        # (a head of another type than the rows: only on the CPU)
+        if top or not self.scores_from_hidden or h.dtype != w.lm_head.dtype or h.dtype not in lops.TYPES:
+            return lops.token_logprobs(lops.widened(self.logits(h, rows)), ids, top)
         if rows is not None:
             h = h.index_select(0, rows)
-        x = self._norm(h, w.final_norm, w.extra.get("final_norm_b"))
-        return lops.head_logprobs(x, w.lm_head, ids, bias=w.extra.get("lm_head_b"), scale=1.0 / float(cfg.extra.get("logits_scaling", 1.0)),
-                                  softcap=float(cfg.final_logit_softcap))
+        x, bias = self._norm(h, w.final_norm, w.extra.get("final_norm_b")), w.extra.get("lm_head_b")
+        return lops.head_logprobs(x, w.lm_head, ids, bias=None if bias is None else lops.widened(bias), softcap=float(cfg.final_logit_softcap),
+                                  scale=1.0 / float(cfg.extra.get("logits_scaling", 1.0)))
 
     def forward(self, b: StepBatch, kv_layers: list[KVLayer]) -> torch.Tensor:
         h = self.forward_hidden(b, kv_layers)

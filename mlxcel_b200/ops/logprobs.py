@@ -10,6 +10,7 @@ import torch
 from . import _lib, linear, reference as ref
 
 MAX_TOP = 64
+TYPES = (torch.bfloat16, torch.float32)           # of logits, hidden rows, weights and biases
 _ARGS = struct.Struct("PqPPPPPPPiiiiiiiff")        # MxTokenLogprobs of csrc/api.h
 # head_logprobs keeps its logits on the chip, unless few rows meet large weights: there both forms read the weights at the pace of the
 # memory, and the smaller tiles of `linear` are the faster ones. us on the chip / through memory: 8 rows, 128256 x 4096 230 / 174, 64
@@ -32,11 +33,16 @@ class TokenLogprobs(NamedTuple):
 def _check(rows: int, vocab: int, device, ids, bias, scale: float, softcap: float, dim: int) -> None:
     if ids.dtype not in (torch.int32, torch.int64) or ids.dim() not in (1, 2)[:dim] or ids.shape[0] != rows or ids.device != device:
         raise ValueError(f"ids have to be int32 or int64 [{rows}]{f' or [{rows}, n]' if dim > 1 else ''} on {device}")
-    if bias is not None and (bias.shape != (vocab,) or bias.dtype not in (torch.bfloat16, torch.float32) or bias.device != device
+    if bias is not None and (bias.shape != (vocab,) or bias.dtype not in TYPES or bias.device != device
                              or not bias.is_contiguous()):
         raise ValueError(f"bias has to be a contiguous bf16 or fp32 [{vocab}] tensor on {device}")
     if not scale > 0.0 or not softcap >= 0.0:
         raise ValueError("scale has to be positive and softcap not negative")
+
+
+def widened(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself, or in fp32 where it is of a type that is not covered here (models on the CPU run in others)."""
+    return t if t.dtype in TYPES else t.float()
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, bias: torch.Tensor | None = None, scale: float = 1.0,
@@ -44,7 +50,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, bia
     """``logits`` [R, V] (bf16 or fp32, rows may be strided) and the tokens asked for, ``ids`` [R] or [R, n]. The distribution is that
     of ``softcap * tanh((logits + bias) * scale / softcap)`` (no cap: 0). NaN counts as -inf; a row with nothing left has log
     probabilities and ``lse`` of -inf and entropy 0; an id outside the vocabulary has log probability NaN. ``top``: up to 64."""
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+    if logits.dim() != 2 or logits.dtype not in TYPES:
         raise ValueError(f"logits have to be bf16 or fp32 [R, V], not {logits.dtype} {tuple(logits.shape)}")
     R, V = logits.shape
     _check(R, V, logits.device, ids, bias, scale, softcap, 2)
@@ -73,7 +79,7 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, *, bias: 
     ``x`` [R, K] and the head's weights ``w`` [V, K] are bf16 (or both fp32); ``ids`` [R]."""
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
         raise ValueError("hidden rows [R, K] and head weights [V, K] of one type are needed on one device")
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dtype not in TYPES:
         raise ValueError(f"hidden rows have to be bf16 or fp32, not {x.dtype}")
     R, V = x.shape[0], w.shape[0]
     _check(R, V, x.device, ids, bias, scale, softcap, 1)

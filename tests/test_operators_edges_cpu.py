@@ -15,7 +15,7 @@ from fastapi.testclient import TestClient
 
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
-from mlxcel_b200.engine.scoring import prefill_hidden
+from mlxcel_b200.engine.scoring import prefill_hidden, sequence_scores
 from mlxcel_b200.models.decoder import DecoderModel
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
@@ -97,6 +97,42 @@ def test_vision_backbone_in_other_types(dtype):
 
 
 # ----------------------------------------------------------------------------- log probabilities of requests
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("top", [0, 3])
+def test_scores_of_models_in_other_types(dtype, top):
+    """The log probabilities of the logits that the model makes, in whatever type: as an fp32 log softmax has them."""
+    ids = [(37 * i) % 1000 for i in range(30)]
+    cfg, model = _tiny(dtype=dtype)
+    want = torch.log_softmax(model.logits(prefill_hidden(model, cfg, ids, 8), torch.arange(29)).float(), -1)
+    got = sequence_scores(model, cfg, ids, 8, top=top)
+    assert torch.allclose(got.logprob, want.gather(1, torch.tensor(ids[1:])[:, None])[:, 0], atol=1e-5)
+    assert got.top_ids.shape == (29, top) and torch.allclose(got.top_logprobs, want.sort(dim=-1, descending=True, stable=True).values[:, :top], atol=1e-5)
+
+    class Bare:                                      # a model that offers logits alone
+        device = model.device
+
+        def logits(self, h, rows):
+            return model.logits(h, rows)
+
+        def __getattr__(self, name):
+            if name == "token_logprobs":
+                raise AttributeError(name)
+            return getattr(model, name)
+    assert all(torch.equal(a, b) for a, b in zip(sequence_scores(Bare(), cfg, ids, 8, top=top), got))
+
+
+def test_scores_with_a_head_or_bias_of_another_type():
+    ids = [(37 * i) % 1000 for i in range(30)]
+    for head, bias in ((torch.float16, None), (torch.bfloat16, None), (None, torch.float16), (None, torch.float64)):
+        cfg, model = _tiny()
+        if head:
+            model.w.lm_head = model.w.lm_head.to(head)
+        if bias:
+            model.w.extra["lm_head_b"] = (torch.randn(cfg.vocab_size, generator=torch.Generator().manual_seed(1)) * 0.5).to(torch.bfloat16).to(bias)
+        want = torch.log_softmax(model.logits(prefill_hidden(model, cfg, ids, 8), torch.arange(29)).double(), -1).gather(1, torch.tensor(ids[1:])[:, None])[:, 0]
+        assert torch.allclose(sequence_scores(model, cfg, ids, 8).logprob.double(), want, atol=1e-4), (head, bias)
 
 
 def test_alternatives_change_no_draw():
@@ -185,7 +221,7 @@ dist.init_process_group("gloo")
 rank, world = dist.get_rank(), dist.get_world_size()
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
-from mlxcel_b200.engine.scoring import prefill_hidden
+from mlxcel_b200.engine.scoring import prefill_hidden, sequence_scores
 from mlxcel_b200.models.decoder import DecoderModel
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
