@@ -263,10 +263,14 @@ class DecoderModel:
             if self._mrope_axes is None:
                 self._mrope_axes = rotary.section_axes(cfg.extra["mrope_section"], rot_dim // 2,
                                                        bool(cfg.extra.get("mrope_interleaved"))).to(qkv.device)
-            rotary.mrope_append(qkv, b.positions3, b.slot_mapping_win if win else b.slot_mapping, self.inv_freq, self._mrope_axes, kv,
-                                Hq=self.Hq, Hkv=self.Hkv, D=self.D, rot_dim=rot_dim, traditional=cfg.rope_traditional,
-                                mscale=self.mscale, q_norm_w=q_norm, k_norm_w=k_norm, norm_eps=cfg.rms_norm_eps,
-                                out=qkv[:, : self.Hq * self.D])
+            args = (qkv, b.positions3, b.slot_mapping_win if win else b.slot_mapping, self.inv_freq, self._mrope_axes, kv)
+            kw = dict(Hq=self.Hq, Hkv=self.Hkv, D=self.D, rot_dim=rot_dim, traditional=cfg.rope_traditional, mscale=self.mscale, q_norm_w=q_norm,
+                      k_norm_w=k_norm, norm_eps=cfg.rms_norm_eps)
+            q = qkv[:, : self.Hq * self.D]
+            if not qkv.is_cuda and any(n is not None and n.dtype != qkv.dtype for n in (q_norm, k_norm)):
+                q.copy_(ops.reference.mrope_append(*args, **kw))         # (norm weights of a type of their own: only on the CPU)
+            else:
+                rotary.mrope_append(*args, **kw, out=q)
             return self._attend(qkv, b, kv, window, lw.sinks, win)
         use_win = window > 0 and b.slot_mapping_win is not None     # this layer's KV lives in the window pool
         ops.rope_append(qkv, b.positions, b.slot_mapping_win if use_win else b.slot_mapping,

@@ -13,10 +13,11 @@ import pytest
 import torch
 from fastapi.testclient import TestClient
 
+from mlxcel_b200.cache.kv_pool import KVPool
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
 from mlxcel_b200.engine.scoring import prefill_hidden, sequence_scores
-from mlxcel_b200.models.decoder import DecoderModel
+from mlxcel_b200.models.decoder import DecoderModel, StepBatch
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.ops import KVLayer, _lib, rotary
@@ -73,6 +74,22 @@ def test_norms_around_sub_layers_in_other_types(extra):
         # 2 layers, each of some 8 roundings to the row type (fp32 within): relative to the spread of the rows
         assert got.dtype == dtype and (got.double() - want).norm() < 16 * max(u, 2.0 ** -20) * want.norm()
     assert torch.equal(hidden(dtype=torch.bfloat16), hidden(dtype=torch.bfloat16, norms=torch.float32))
+
+
+def test_image_positions_with_head_norms_of_another_type():
+    """bf16 rows whose per-head norm weights are the same numbers in fp32."""
+    def run(norms):
+        cfg, model = _tiny(dtype=torch.bfloat16, mrope_section=[12, 10, 10])
+        for lw in model.w.layers:
+            lw.q_norm, lw.k_norm = (1.0 + torch.arange(64) / 64).to(norms), (2.0 - torch.arange(64) / 64).to(norms)
+        T, i32 = 9, dict(dtype=torch.int32)
+        pool = KVPool(cfg, 2, 8, dtype=torch.bfloat16)
+        b = StepBatch(token_ids=torch.arange(3, 3 + T, **i32), positions=torch.arange(T, **i32), slot_mapping=torch.arange(T, **i32), num_prefill_seqs=1,
+                      pf_block_tables=torch.arange(2, **i32)[None], pf_cu_q=torch.tensor([0, T], **i32), pf_context_lens=torch.tensor([T], **i32),
+                      pf_max_q_len=T, pf_max_len=T, pf_cu_q_host=[0, T], logits_rows=torch.arange(T))
+        b.positions3 = torch.stack([torch.arange(T), torch.arange(T) // 3, torch.arange(T) % 3]).int()
+        return model.forward(b, pool.layers)
+    assert torch.equal(run(torch.bfloat16), run(torch.float32))
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
@@ -219,10 +236,11 @@ import sys, torch, torch.distributed as dist
 sys.path.insert(0, %r)
 dist.init_process_group("gloo")
 rank, world = dist.get_rank(), dist.get_world_size()
+from mlxcel_b200.cache.kv_pool import KVPool
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
 from mlxcel_b200.engine.scoring import prefill_hidden, sequence_scores
-from mlxcel_b200.models.decoder import DecoderModel
+from mlxcel_b200.models.decoder import DecoderModel, StepBatch
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.loading.shard import shard_weights, partition_layers
