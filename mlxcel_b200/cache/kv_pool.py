@@ -147,14 +147,29 @@ class KVPool:
         return out
 
     def restore_blocks(self, block_ids: list[int], data: list[dict]) -> None:
-        """Puts what :meth:`extract_blocks` returned into blocks, each named once."""
+        """Puts what :meth:`extract_blocks` returned into blocks, each named once. Layers and slabs that ``data`` lacks stay as they are;
+        blocks of another pool's layout are refused, and nothing has moved then."""
         slabs, n = self.page_slabs(), len(block_ids)
         if n == 0:
             return
-        rows = [data[i][name] for i, name in self._slab_names() if getattr(self.layers[i], name).numel()]
+        if any(getattr(l, name) is None for l, d in zip(self.layers, data) for name in d):
+            raise ValueError("the blocks have slabs that this pool lacks")
+        rows: list[torch.Tensor | None] = []
+        for i, name in self._slab_names():
+            t, src = getattr(self.layers[i], name), data[i].get(name) if i < len(data) else None
+            if src is not None and (src.shape[1:] != t.shape[1:] or src.shape[0] not in (1, n) or (src.dtype == torch.uint8) != (t.dtype == torch.uint8)):
+                raise ValueError(f"layer {i}: {name} of {src.dtype} {tuple(src.shape)} are no {n} blocks of {t.dtype} {tuple(t.shape[1:])}")
+            if t.numel():
+                rows.append(src)
         for first, end in self._batches(n):
-            buf, at = torch.empty(n * sum(slabs.page_bytes[first:end]), dtype=torch.uint8, device=slabs.device), 0
-            for t, size, src in zip(slabs.slabs[first:end], slabs.page_bytes[first:end], rows[first:end]):
-                buf[at:at + size * n].view(t.dtype).view(n, *t.shape[1:]).copy_(src)
-                at += size * n
-            slabs.scatter(block_ids, buf, first=first, count=end - first)
+            while first < end:                                # runs of slabs that are there
+                last = first
+                while last < end and rows[last] is not None:
+                    last += 1
+                if last > first:
+                    buf, at = torch.empty(n * sum(slabs.page_bytes[first:last]), dtype=torch.uint8, device=slabs.device), 0
+                    for t, size, src in zip(slabs.slabs[first:last], slabs.page_bytes[first:last], rows[first:last]):
+                        buf[at:at + size * n].view(t.dtype).view(n, *t.shape[1:]).copy_(src)
+                        at += size * n
+                    slabs.scatter(block_ids, buf, first=first, count=last - first)
+                first = last + 1

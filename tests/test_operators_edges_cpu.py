@@ -13,6 +13,7 @@ import pytest
 import torch
 from fastapi.testclient import TestClient
 
+from mlxcel_b200.cache import kv_pool
 from mlxcel_b200.cache.kv_pool import KVPool
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
@@ -41,6 +42,48 @@ def test_mrope_entry_refuses_no_heads_before_it_launches():
     """The C entry checks this itself (it returns before it asks for a device)."""
     args = rotary._ARGS.pack(*([16, 0] * 3), 16, 16, 64, *[16] * 5, 0, 0, 3, 5, 0, 0, 64, 64, 16, 0, 16, 1e-6, 1.0)
     assert len(args) == struct.calcsize(rotary._ARGS.format) and _lib.load().mx_mrope_append(args, None) == -1
+
+
+# ----------------------------------------------------------------------------- pages of the pool
+@pytest.mark.parametrize("limit", [1 << 30, 5000, 1])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_pool_restores_what_a_snapshot_has(bits, limit, monkeypatch):
+    monkeypatch.setattr(kv_pool, "STAGING_BYTES", limit)
+    cfg = copy.deepcopy(preset("tiny-llama"))
+    cfg.num_hidden_layers = 4
+    pool, g = KVPool(cfg, 6, 8, kv_bits=bits, dtype=torch.float32), torch.Generator().manual_seed(1)
+    slabs = [(i, n) for i, l in enumerate(pool.layers) for n in kv_pool.SLABS if getattr(l, n) is not None]
+    for i, n in slabs:
+        t = getattr(pool.layers[i], n)
+        t.copy_(torch.randint(1, 200, t.shape, generator=g).to(t.dtype))
+    data = pool.extract_blocks([5, 1])
+    whole = [dict(d) for d in data]
+    del data[1]["v"], data[2]["k"], data[3]                    # slabs and a layer are not there
+    other = KVPool(cfg, 6, 8, kv_bits=bits, dtype=torch.float32)
+    other.restore_blocks([0, 4], data)
+    for i, n in slabs:
+        t = getattr(other.layers[i], n)
+        there = i < len(data) and n in data[i]
+        assert torch.equal(t[[0, 4]], whole[i][n] if there else torch.zeros_like(whole[i][n])) and not t[[1, 2, 3, 5]].any()
+    other.restore_blocks([2, 3], [])
+    assert not any(getattr(l, n)[[2, 3]].any() for l in other.layers for n in kv_pool.SLABS if getattr(l, n) is not None)
+
+
+def test_pool_refuses_blocks_of_another_layout():
+    cfg = preset("tiny-llama")
+    pools = {bits: KVPool(cfg, 4, 8, kv_bits=bits, dtype=torch.float32) for bits in (16, 8, 4)}
+    snaps = {bits: p.extract_blocks([1, 2]) for bits, p in pools.items()}
+    for to, p in pools.items():
+        for t in (getattr(l, n) for l in p.layers for n in kv_pool.SLABS if getattr(l, n) is not None):
+            t.fill_(3)
+        for frm, s in snaps.items():
+            if frm != to:
+                with pytest.raises(ValueError):
+                    p.restore_blocks([0, 3], s)
+        for bad in ([0], [0, 1, 2]):                           # another number of blocks than the snapshot has
+            with pytest.raises(ValueError):
+                p.restore_blocks(bad, snaps[to])
+        assert all((getattr(l, n) == 3).all() for l in p.layers for n in kv_pool.SLABS if getattr(l, n) is not None)
 
 
 # ----------------------------------------------------------------------------- models of other types
@@ -236,6 +279,7 @@ import sys, torch, torch.distributed as dist
 sys.path.insert(0, %r)
 dist.init_process_group("gloo")
 rank, world = dist.get_rank(), dist.get_world_size()
+from mlxcel_b200.cache import kv_pool
 from mlxcel_b200.cache.kv_pool import KVPool
 from mlxcel_b200.config import preset
 from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
