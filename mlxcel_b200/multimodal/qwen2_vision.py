@@ -11,6 +11,7 @@ position; text after the image continues at ``max(position) + 1``.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -96,12 +97,13 @@ class _AxialHeads:
         half = self.dim // self.heads // 2
         inv = torch.cat([self.inv_freq, self.inv_freq]).to(self.device)
         axes = (torch.arange(half) >= half // 2).int().to(self.device)
-        # (projections in fp32 on a GPU take the plain statement: the kernel reads bf16)
-        plain = self.device.type == "cuda" and self.dtype != torch.bfloat16
-        turn = lambda z: ops.reference.rotate_axes(z, pos, inv, axes, 2 * half)    # noqa: E731
-        if plain:
-            return lambda qkv: ops.reference.axial_rope(qkv, pos, inv, axes, self.heads, 2 * half), turn
-        return lambda qkv: rotary.axial_rope(qkv, pos, inv, axes, heads=self.heads, D=2 * half), turn
+        angles = functools.cache(lambda: ops.reference.axes_angles(pos, inv, axes, half))      # (of all blocks)
+        # on the CPU, and for projections of other types than the kernel reads, the plain statement
+        if self.device.type != "cuda" or self.dtype != torch.bfloat16:
+            heads = lambda qkv: ops.reference.turned_heads(qkv, *angles(), self.heads)    # noqa: E731
+        else:
+            heads = lambda qkv: rotary.axial_rope(qkv, pos, inv, axes, heads=self.heads, D=2 * half)    # noqa: E731
+        return heads, lambda z: ops.reference.turn_heads(z, *angles())
 
 
 class Qwen2VisionTower(_AxialHeads):

@@ -201,22 +201,31 @@ def section_axes(sections, half: int, interleaved: bool = False) -> torch.Tensor
     return which
 
 
-def rotate_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, axes: torch.Tensor, rot_dim: int,
-                traditional: bool = False, mscale: float = 1.0) -> torch.Tensor:
-    """x [T, H, D] → fp32 with the first ``rot_dim`` columns of each head turned, frequency i by ``positions[axes[i]]``. Angles in
-    64 bits: an fp32 product of a far position is off by hundredths of a radian."""
-    half = rot_dim // 2
-    out = x.float().clone()
-    if half == 0:
-        return out
+def axes_angles(positions: torch.Tensor, inv_freq: torch.Tensor, axes: torch.Tensor, half: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cosine and sine [T, half], fp32, of frequency i turning by ``positions[axes[i]]``. Angles in 64 bits: an fp32 product of a far
+    position is off by hundredths of a radian."""
     which = axes[:half].long().clamp(0, positions.shape[0] - 1)
     ang = positions.double().t()[:, which] * inv_freq[:half].double()
-    cos, sin = ang.cos().float()[:, None], ang.sin().float()[:, None]
-    first, second = (slice(0, rot_dim, 2), slice(1, rot_dim, 2)) if traditional else (slice(0, half), slice(half, rot_dim))
-    a, b = out[..., first].clone(), out[..., second].clone()
-    out[..., first] = (a * cos - b * sin) * mscale
-    out[..., second] = (b * cos + a * sin) * mscale
-    return out
+    return ang.cos().float(), ang.sin().float()
+
+
+def turn_heads(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, traditional: bool = False, mscale: float = 1.0) -> torch.Tensor:
+    """x [T, H, D] → fp32 with the first columns of each head, two for each of the angles of :func:`axes_angles`, turned."""
+    x, half = x.float(), cos.shape[1]
+    cos, sin = cos[:, None] * mscale, sin[:, None] * mscale
+    if traditional:
+        a, b = x[..., 0:2 * half:2], x[..., 1:2 * half:2]
+        turned = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+    else:
+        a, b = x[..., :half], x[..., half:2 * half]
+        turned = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+    return turned if 2 * half == x.shape[-1] else torch.cat([turned, x[..., 2 * half:]], dim=-1)
+
+
+def rotate_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, axes: torch.Tensor, rot_dim: int,
+                traditional: bool = False, mscale: float = 1.0) -> torch.Tensor:
+    """x [T, H, D] → fp32 with the first ``rot_dim`` columns of each head turned, frequency i by ``positions[axes[i]]``."""
+    return turn_heads(x, *axes_angles(positions, inv_freq, axes, rot_dim // 2), traditional, mscale)
 
 
 def mrope_append(qkv, positions, slot_mapping, inv_freq, axes, kv, *, Hq, Hkv, D, rot_dim, traditional=False, mscale=1.0,
@@ -240,9 +249,13 @@ def mrope_append(qkv, positions, slot_mapping, inv_freq, axes, kv, *, Hq, Hkv, D
 
 def axial_rope(qkv, positions, inv_freq, axes, heads: int, D: int):
     """Plain statement of ``ops.rotary.axial_rope``."""
-    x = qkv.view(qkv.shape[0], 3, heads, D)
-    turn = lambda t: rotate_axes(t, positions, inv_freq, axes, D).transpose(0, 1).contiguous()    # noqa: E731
-    return turn(x[:, 0]), turn(x[:, 1]), x[:, 2].float().transpose(0, 1).contiguous()
+    return tuple(t.contiguous() for t in turned_heads(qkv, *axes_angles(positions, inv_freq, axes, D // 2), heads))
+
+
+def turned_heads(qkv, cos, sin, heads: int):
+    """:func:`axial_rope` with the angles of :func:`axes_angles` (one forward's, for all its blocks), as views of any order."""
+    q, k, v = qkv.view(qkv.shape[0], 3, heads, -1).unbind(1)
+    return turn_heads(q, cos, sin).transpose(0, 1), turn_heads(k, cos, sin).transpose(0, 1), v.float().transpose(0, 1)
 
 
 def branch_norm(x, residual, post_w, gate, scale: float, pre_w, pre_b, layer_norm: bool, eps: float, w_bias: float):

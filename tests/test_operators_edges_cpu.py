@@ -21,6 +21,7 @@ from mlxcel_b200.engine.scoring import prefill_hidden, sequence_scores
 from mlxcel_b200.models.decoder import DecoderModel, StepBatch
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
+from mlxcel_b200.multimodal.qwen2_vision import Glm4vVisionTower, Qwen2VisionTower
 from mlxcel_b200.ops import KVLayer, _lib, rotary
 from mlxcel_b200.server.app import ServerState, create_app
 from mlxcel_b200.server.worker import ModelWorker
@@ -154,6 +155,59 @@ def test_vision_backbone_in_other_types(dtype):
     want = Dinov2Backbone(cfg, t, dtype=torch.float32).forward(x)[0].double()
     got = Dinov2Backbone(cfg, t, dtype=dtype).forward(x)[0]
     assert got.dtype == dtype and (got.double() - want).norm() < 24 * 2.0 ** -11 * want.norm()
+
+
+def _tower(kind, dim=64, heads=2, dtype=torch.float32, device="cpu", blocks=3, head_norms=True):
+    """A small tower of random weights: Qwen2-VL's, or GLM-4V's (with norms of the heads, GLM-OCR's)."""
+    g = torch.Generator().manual_seed(0)
+    rn = lambda *s: torch.randn(*s, generator=g) * 0.2    # noqa: E731
+    t = {"patch_embed.proj.weight": rn(dim, 3, 2, 2, 2)}
+    if kind is Qwen2VisionTower:
+        for n in ("merger.ln_q", *(f"blocks.{i}.norm{j}" for i in range(blocks) for j in (1, 2))):
+            t[n + ".weight"], t[n + ".bias"] = 1 + rn(dim), rn(dim)
+        shapes = [(f"blocks.{i}.{n}", s) for i in range(blocks) for n, s in (("attn.qkv", (3 * dim, dim)), ("attn.proj", (dim, dim)), ("mlp.fc1", (2 * dim, dim)),
+                                                                            ("mlp.fc2", (dim, 2 * dim)))]
+        for n, s in shapes + [("merger.mlp.0", (4 * dim, 4 * dim)), ("merger.mlp.2", (dim, 4 * dim))]:
+            t[n + ".weight"], t[n + ".bias"] = rn(*s), rn(s[0])
+        return kind(dict(depth=blocks, embed_dim=dim, num_heads=heads, patch_size=2), t, dtype, device)
+    t.update({"patch_embed.proj.bias": rn(dim), "post_layernorm.weight": 1 + rn(dim), "downsample.weight": rn(dim, dim, 2, 2), "downsample.bias": rn(dim),
+              "merger.proj.weight": rn(dim, dim), "merger.post_projection_norm.weight": 1 + rn(dim), "merger.post_projection_norm.bias": rn(dim),
+              "merger.gate_proj.weight": rn(dim, dim), "merger.up_proj.weight": rn(dim, dim), "merger.down_proj.weight": rn(dim, dim)})
+    for i in range(blocks):
+        b = f"blocks.{i}."
+        t.update({b + "norm1.weight": 1 + rn(dim), b + "norm2.weight": 1 + rn(dim), b + "attn.qkv.weight": rn(3 * dim, dim), b + "attn.proj.weight": rn(dim, dim),
+                  b + "mlp.gate_proj.weight": rn(dim, dim), b + "mlp.up_proj.weight": rn(dim, dim), b + "mlp.down_proj.weight": rn(dim, dim)})
+        if head_norms:
+            t.update({b + "attn.q_norm.weight": 1 + rn(dim // heads), b + "attn.k_norm.weight": 1 + rn(dim // heads)})
+    return kind(dict(depth=blocks, hidden_size=dim, num_heads=heads, patch_size=2), t, dtype, device)
+
+
+@pytest.mark.parametrize("kind,head_norms", [(Qwen2VisionTower, False), (Glm4vVisionTower, True), (Glm4vVisionTower, False)])
+def test_towers_make_their_angles_once(kind, head_norms, monkeypatch):
+    """The cosines of a forward are those of its grids, for all blocks, and the rows are those of angles made at every use."""
+    tower, grids = _tower(kind, head_norms=head_norms), [(1, 4, 6), (1, 2, 2)]
+    rows = torch.randn(28, 24, generator=torch.Generator().manual_seed(1))
+    calls, cos = [], torch.Tensor.cos
+    monkeypatch.setattr(torch.Tensor, "cos", lambda t: (calls.append(t.shape), cos(t))[1])
+    got = tower.forward(rows, grids)
+    assert len(calls) == 1
+    # written out: each block's q and k turned as pairs (i, i + 16), i < 8 by the patch's row, else by its column
+    angles = []
+    for _, gh, gw in grids:
+        hp = torch.arange(gh)[:, None].expand(gh, gw).reshape(gh // 2, 2, gw // 2, 2).permute(0, 2, 1, 3).flatten()
+        wp = torch.arange(gw)[None].expand(gh, gw).reshape(gh // 2, 2, gw // 2, 2).permute(0, 2, 1, 3).flatten()
+        angles.append(torch.cat([hp[:, None] * tower.inv_freq, wp[:, None] * tower.inv_freq], 1))
+    c, s = (f(torch.cat(angles).double()).repeat(1, 2).float()[:, None] for f in (torch.cos, torch.sin))
+
+    def turn(z):
+        return z * c + torch.cat([-z[..., 16:], z[..., :16]], -1) * s
+
+    def heads(qkv):
+        q, k, v = qkv.view(28, 3, 2, 32).float().unbind(1)
+        return [z.transpose(0, 1) for z in (turn(q), turn(k), v)]
+    tower._axial = lambda grids: (heads, turn)
+    want = tower.forward(rows, grids)
+    assert torch.allclose(got, want, atol=1e-4 * want.abs().max().item())
 
 
 # ----------------------------------------------------------------------------- log probabilities of requests
