@@ -98,8 +98,8 @@ class _AxialHeads:
         inv = torch.cat([self.inv_freq, self.inv_freq]).to(self.device)
         axes = (torch.arange(half) >= half // 2).int().to(self.device)
         angles = functools.cache(lambda: ops.reference.axes_angles(pos, inv, axes, half))      # (of all blocks)
-        # on the CPU, and for projections of other types than the kernel reads, the plain statement
-        if self.device.type != "cuda" or self.dtype != torch.bfloat16:
+        # on the CPU, and for types and head sizes that the kernel does not take, the plain statement
+        if self.device.type != "cuda" or self.dtype != torch.bfloat16 or 2 * half > rotary.MAX_DIM:
             heads = lambda qkv: ops.reference.turned_heads(qkv, *angles(), self.heads)    # noqa: E731
         else:
             heads = lambda qkv: rotary.axial_rope(qkv, pos, inv, axes, heads=self.heads, D=2 * half)    # noqa: E731

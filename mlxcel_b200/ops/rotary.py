@@ -11,6 +11,7 @@ import torch
 
 from . import KVLayer, _lib, reference as ref
 
+MAX_DIM = 256                                             # of a head, on the GPU
 _ARGS = struct.Struct("PqPqPqPPqPPPPPPPiiiiiiiiiff")        # MxMropeAppend of csrc/api.h
 
 
@@ -69,8 +70,8 @@ def mrope_append(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch
         q = ref.mrope_append(qkv, positions, slot_mapping, inv_freq, axes, kv, Hq=Hq, Hkv=Hkv, D=D, rot_dim=rot_dim,
                              traditional=traditional, mscale=mscale, q_norm_w=q_norm_w, k_norm_w=k_norm_w, norm_eps=norm_eps)
         return q if out is None else out.copy_(q)
-    if dtype != torch.bfloat16 or D > 256:
-        raise ValueError(f"the kernel takes bf16 projections with heads of up to 256, not {dtype} with {D}")
+    if dtype != torch.bfloat16 or D > MAX_DIM:
+        raise ValueError(f"the kernel takes bf16 projections with heads of up to {MAX_DIM}, not {dtype} with {D}")
     ldqkv, one = qkv.stride()
     ldq, one_q = (Hq * D, 1) if out is None else out.stride()
     if one != 1 or one_q != 1 or T > 1 and (ldqkv < width or ldq < Hq * D):
@@ -103,8 +104,8 @@ def axial_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     _check_angles(positions, axes, inv_freq, D // 2, R, qkv.get_device())
     if not qkv.is_cuda:
         return ref.axial_rope(qkv, positions, inv_freq, axes, heads, D)
-    if qkv.dtype != torch.bfloat16 or D > 256:
-        raise ValueError(f"the kernel takes bf16 projections with heads of up to 256, not {qkv.dtype} with {D}")
+    if qkv.dtype != torch.bfloat16 or D > MAX_DIM:
+        raise ValueError(f"the kernel takes bf16 projections with heads of up to {MAX_DIM}, not {qkv.dtype} with {D}")
     if qkv.stride(1) != 1 or R > 1 and (qkv.stride(0) < qkv.shape[1] or positions.stride(1) != 1):
         raise ValueError("the elements of a row and an axis' positions have to be adjacent")
     q, k, v = qkv.new_empty((3, heads, R, D), dtype=torch.float32).unbind()

@@ -39,3 +39,18 @@ def test_axial_entry_with_results_off_16_bytes(off):
         # (two kernels with one formula each: their products and sums may be contracted differently, half a step of each term)
         assert ((g.view(H, R, D) - w).abs() <= 2.0 ** -22 * w.abs().amax().clamp(min=1.0)).all()
         assert not f[:o].any() and not f[o + R * H * D:].any()
+
+
+@pytest.mark.parametrize("head_norms", [False, True])
+@pytest.mark.parametrize("dim,heads", [(528, 2), (128, 2)])
+def test_tower_on_the_gpu_against_the_cpu(dim, heads, head_norms):
+    """GLM-4V's tower with and without norms of the heads, whose heads the kernel takes (64) and does not (264), bf16 against fp32."""
+    from test_operators_edges_cpu import Glm4vVisionTower, _tower
+    kw = dict(head_norms=head_norms, scale=dim ** -0.5)
+    grids, rows = [(1, 4, 6), (1, 2, 2)], torch.randn(28, 24, generator=torch.Generator().manual_seed(1))
+    want = _tower(Glm4vVisionTower, dim, heads, **kw).forward(rows, grids).double()
+    got = _tower(Glm4vVisionTower, dim, heads, torch.bfloat16, DEV, **kw).forward(rows, grids)
+    assert got.dtype == torch.bfloat16
+    # weights and inputs rounded to bf16, then some 10 rounded steps in each of 3 blocks and 8 behind them: each moves the rows by up to
+    # 2^-8 of their size, at random; twice the root of their number
+    assert (got.double().cpu() - want).norm() < 2 * 48 ** 0.5 * 2.0 ** -8 * want.norm()

@@ -157,10 +157,10 @@ def test_vision_backbone_in_other_types(dtype):
     assert got.dtype == dtype and (got.double() - want).norm() < 24 * 2.0 ** -11 * want.norm()
 
 
-def _tower(kind, dim=64, heads=2, dtype=torch.float32, device="cpu", blocks=3, head_norms=True):
+def _tower(kind, dim=64, heads=2, dtype=torch.float32, device="cpu", blocks=3, head_norms=True, scale=0.2):
     """A small tower of random weights: Qwen2-VL's, or GLM-4V's (with norms of the heads, GLM-OCR's)."""
     g = torch.Generator().manual_seed(0)
-    rn = lambda *s: torch.randn(*s, generator=g) * 0.2    # noqa: E731
+    rn = lambda *s: torch.randn(*s, generator=g) * scale    # noqa: E731
     t = {"patch_embed.proj.weight": rn(dim, 3, 2, 2, 2)}
     if kind is Qwen2VisionTower:
         for n in ("merger.ln_q", *(f"blocks.{i}.norm{j}" for i in range(blocks) for j in (1, 2))):
