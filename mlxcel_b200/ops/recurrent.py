@@ -271,6 +271,8 @@ def layernorm(x, weight, bias=None, eps: float = 1e-5):
     if not x.is_cuda:
         return F.layer_norm(x.float(), (x.shape[-1],), weight.float(), None if bias is None else bias.float(),
                             eps).to(x.dtype)
+    if any(t is not None and t.dtype != torch.bfloat16 for t in (x, weight, bias)):
+        raise ValueError("the kernel takes bf16 rows, weights and biases, not " + ", ".join(str(t.dtype) for t in (x, weight, bias) if t is not None))
     x = x.contiguous()
     y = torch.empty_like(x)
     _call("mx_layernorm", x.data_ptr(), weight.data_ptr(), _lib.ptr(bias), y.data_ptr(), x.shape[0], x.shape[1],

@@ -3,7 +3,7 @@ probabilities take, and the forms that their dispatch chooses for large calls.""
 import pytest
 import torch
 
-from mlxcel_b200.ops import _lib, rotary
+from mlxcel_b200.ops import _lib, recurrent, rotary
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -19,6 +19,15 @@ def _status_clean():
 def _rn(*shape, seed=0, scale=1.0, shift=0.0, dtype=torch.bfloat16):
     g = torch.Generator(device=DEV).manual_seed(seed)
     return (torch.randn(*shape, generator=g, device=DEV) * scale + shift).to(dtype)
+
+
+# ----------------------------------------------------------------------------- norms
+def test_layernorm_refuses_types_that_its_kernel_would_misread():
+    x, w, b = _rn(3, 64, seed=1), _rn(64, seed=2), _rn(64, seed=3)
+    assert recurrent.layernorm(x, w, b).dtype == torch.bfloat16
+    for bad in ((x.float(), w, b), (x, w.float(), b), (x, w, b.half()), (x.half(), w.half(), None)):
+        with pytest.raises(ValueError):
+            recurrent.layernorm(*bad)
 
 
 # ----------------------------------------------------------------------------- rotary positions
