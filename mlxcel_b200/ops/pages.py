@@ -18,7 +18,7 @@ def _list(ids) -> list:
 
 
 class PageSlabs:
-    """The slabs of a pool, [pages, ...] each, in the order in which a buffer holds them. Page ids are host lists (or CPU tensors and
+    """The slabs of a pool, [pages, ...] each, apart in memory, in the order in which a buffer holds them. Page ids are host lists (or CPU tensors and
     arrays) and are checked: a page outside the pool, a destination named twice or a source missing raises ``ValueError`` and moves
     nothing. Slabs whose pages are empty are left out. The ids of small calls (106 copies, 320 pages) travel with the launch, which can
     be captured into a graph; longer tables are copied to the device first, which cannot."""
@@ -31,6 +31,9 @@ class PageSlabs:
             if t.shape[0] != self.num_pages or t.device != self.device or not t.is_contiguous():
                 raise ValueError("slabs have to be contiguous, on one device and of as many pages each")
         self.slabs = [t for t in slabs if t.numel()]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.slabs)
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("slabs have to lie apart: bytes that two of them share would move twice")
         self.page_bytes = [t[0].numel() * t.element_size() for t in self.slabs]
         self.bytes_per_page = sum(self.page_bytes)
         n = len(self.slabs)

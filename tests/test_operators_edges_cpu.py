@@ -22,7 +22,7 @@ from mlxcel_b200.models.decoder import DecoderModel, StepBatch
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.multimodal.qwen2_vision import Glm4vVisionTower, Qwen2VisionTower
-from mlxcel_b200.ops import KVLayer, _lib, rotary
+from mlxcel_b200.ops import KVLayer, _lib, pages, rotary
 from mlxcel_b200.server.app import ServerState, create_app
 from mlxcel_b200.server.worker import ModelWorker
 from mlxcel_b200.tokenizer import ByteTokenizer
@@ -46,6 +46,17 @@ def test_mrope_entry_refuses_no_heads_before_it_launches():
 
 
 # ----------------------------------------------------------------------------- pages of the pool
+def test_slabs_that_share_memory_are_refused():
+    """A chain of copies would be taken once per slab: pages 0, 1, 2 in place of 0, 0, 1 became 0, 0, 0."""
+    t, wide = torch.arange(12).view(4, 3), torch.arange(24)
+    for bad in ([t, t], [t, t.view(4, 3)], [wide[:12].view(4, 3), wide[9:21].view(4, 3)], [wide[:8].view(4, 2), torch.zeros(4, 1), wide[7:11].view(4, 1)]):
+        with pytest.raises(ValueError):
+            pages.PageSlabs(bad)
+    near = [wide[:12].view(4, 3), torch.zeros(4, 0), wide[12:].view(4, 3)]                    # (side by side is apart)
+    pages.PageSlabs(near).copy([0, 1], [1, 2])
+    assert wide.view(8, 3)[:, 0].tolist() == [0, 0, 3, 9, 12, 12, 15, 21]
+
+
 @pytest.mark.parametrize("limit", [1 << 30, 5000, 1])
 @pytest.mark.parametrize("bits", [16, 8])
 def test_pool_restores_what_a_snapshot_has(bits, limit, monkeypatch):
