@@ -520,9 +520,13 @@ def create_app(state: ServerState) -> FastAPI:
             many = min(max(0, sp.top_logprobs), MAX_TOP, eng.cfg.vocab_size)       # alternatives at every place
 
             def score():
-                r = sequence_scores(eng.model, eng.cfg, ids, eng.ecfg.block_size, top=many)
+                # (between two steps of the engine: a model's forward keeps its sums of squares and its latest hidden rows in buffers of its own)
+                r = state.worker.run_exclusive(lambda: sequence_scores(eng.model, eng.cfg, ids, eng.ecfg.block_size, top=many))
                 return r.logprob.tolist(), [_ranked(zip(i, v)) for i, v in zip(r.top_ids.tolist(), r.top_logprobs.tolist())] if many else []
-            plp, ptop = await asyncio.get_running_loop().run_in_executor(None, score)
+            try:
+                plp, ptop = await asyncio.get_running_loop().run_in_executor(None, score)
+            except (RuntimeError, ValueError) as e:
+                return _err(400, str(e))
             ptoks = [tk.decode([t], skip_special_tokens=False) for t in ids]
             offs, pos = [], 0
             for piece in ptoks:

@@ -8,6 +8,7 @@ import struct
 import subprocess
 import sys
 import textwrap
+import threading
 
 import pytest
 import torch
@@ -321,6 +322,14 @@ def test_echo_without_log_probabilities_of_generated_tokens(client):
     e = _complete(client, echo=True, top_logprobs=4)
     assert len(e["top_logprobs"]) == len(e["token_logprobs"]) == len(e["tokens"])
     assert e["top_logprobs"][-3:] == e["token_logprobs"][-3:] == [None] * 3 and all(e["top_logprobs"][1:-3])
+
+
+def test_echo_scores_between_steps_of_the_engine(client, monkeypatch):
+    """A forward of the model beside the engine's would share the buffers that both keep in the model: one thread makes both."""
+    threads, forward = [], DecoderModel.forward_hidden
+    monkeypatch.setattr(DecoderModel, "forward_hidden", lambda self, *a, **k: (threads.append(threading.current_thread()), forward(self, *a, **k))[1])
+    _complete(client, echo=True, logprobs=True)
+    assert len(threads) >= 4 and len(set(threads)) == 1
 
 
 def test_a_number_of_log_probabilities_gives_alternatives_without_echo_too(client):
