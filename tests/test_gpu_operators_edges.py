@@ -211,3 +211,26 @@ def test_vision_backbone_in_bf16_against_the_cpu():
         # some 12 steps a block and 3 around them round the rows to bf16 (half a step, 2^-8, of their size), at random: twice the root
         assert a.dtype == torch.bfloat16 and a.shape == b.shape
         assert (a.double().cpu() - b.double()).norm() < 2 * math.sqrt(12 * depth + 3) * 2.0 ** -8 * b.double().norm()
+
+
+def test_alternatives_change_no_draw():
+    """Seeded requests of a mixed batch draw the same tokens, with the same log probabilities, whether or not they ask for alternatives."""
+    from test_gpu_operators_models import _models
+
+    from mlxcel_b200.engine import Engine, EngineConfig, SamplingParams
+    cfg, (_, gpu) = _models()
+    base = [dict(temperature=0.9, top_p=0.9, seed=3), dict(temperature=1.3, top_k=50, seed=4), dict(temperature=0.7, min_p=0.05, seed=5), dict(temperature=0.0)]
+
+    def run(tops):
+        eng = Engine(gpu, cfg, EngineConfig(max_batch=4, max_num_batched_tokens=64, num_blocks=32, max_model_len=128))
+        sids = [eng.add_request([5, 6, 7, 8 + i], SamplingParams(max_tokens=8, ignore_eos=True, logprobs=True, top_logprobs=t, **b))
+                for i, (b, t) in enumerate(zip(base, tops))]
+        while eng.has_work():
+            eng.step()
+        return [eng.seqs[s] for s in sids]
+    want = run([0] * 4)
+    for tops in ([5] * 4, [0, 64, 0, 1]):
+        for s, w, t in zip(run(tops), want, tops):
+            assert s.output == w.output and [len(getattr(lp, "top", [])) for lp in s.logprobs] == [t] * 8
+            # (the sampler's normaliser and the alternatives': fp32 sums of the same logits)
+            assert all(abs(a - b) <= 1e-5 * (1 + abs(b)) for a, b in zip(s.logprobs, w.logprobs))
