@@ -114,8 +114,8 @@ class KVPool:
         return h[1]
 
     def copy_blocks(self, pairs: list[tuple[int, int]]) -> None:
-        """Copies block contents ``src -> dst`` in every layer (copy-on-write, forks, compaction): every block named as a destination,
-        once, becomes what its source was before the call, also where blocks are both."""
+        """Copies block contents ``src -> dst`` in every layer, for users of the pool (the engine shares full blocks and copies none): every
+        block named as a destination, once, becomes what its source was before the call, also where blocks are both."""
         if pairs:
             self.page_slabs().copy([p[0] for p in pairs], [p[1] for p in pairs])
 
@@ -157,7 +157,8 @@ class KVPool:
         rows: list[torch.Tensor | None] = []
         for i, name in self._slab_names():
             t, src = getattr(self.layers[i], name), data[i].get(name) if i < len(data) else None
-            if src is not None and (src.shape[1:] != t.shape[1:] or src.shape[0] not in (1, n) or (src.dtype == torch.uint8) != (t.dtype == torch.uint8)):
+            if src is not None and (src.shape[1:] != t.shape[1:] or src.shape[0] not in (1, n)
+                                    or (src.dtype == torch.uint8) != (t.dtype == torch.uint8)):
                 raise ValueError(f"layer {i}: {name} of {src.dtype} {tuple(src.shape)} are no {n} blocks of {t.dtype} {tuple(t.shape[1:])}")
             if t.numel():
                 rows.append(src)

@@ -4,12 +4,15 @@
 // The products run as in gemm_pair.cu: 256 x 256 tiles on pairs of SMs, operands by TMA, accumulators in TMEM, double-buffered. The
 // epilogue leaves a tile as the sums of its columns per row (m, s, t of logprobs.cuh, one set per half of the tile) in place of 256
 // logits, and the row's own token's logit where the tile holds it. A second launch joins the column tiles of each row.
-// Logits of 2047 rows over 128256 tokens would be 1 GB of fp32; what is written instead is 12 MB. The logits are never rounded.
+// Logits of 2047 rows over 128256 tokens would be 1 GB of fp32; what is written instead is 25 MB (three numbers per row and half tile).
+// The logits are never rounded.
 //
 // Bound by the tensor cores under the power cap: a tile's products take 8 K cycles an SM, its epilogue about 3000 beside them, whose
 // instructions cost power and with it clock. Measured, in a row (us): 2047 rows, K 4096, V 128256 1870 (1.15 PFLOP/s); the same product
 // by gemm_pair.cu, which writes 525 MB of bf16 logits, 1750, by cuBLAS 1550. With the sums left in the tensor core over all of K 1790,
-// and 3e-6 from the 64-bit result in place of 7e-7; with the changes of SHAPED made in any case 120 more.
+// and 3e-6 from the 64-bit result in place of 7e-7; with the changes of SHAPED made in any case 120 more. A tile is 256 rows whatever is
+// left of them, which is what few rows and remainders cost: 256 rows 235 (floor 194), 300 rows 414 (227), 8 to 192 rows of K 1024, V 50257
+// 40 to 42 (16). 168 registers a thread, 40 bytes of them spilled (44 where SHAPED).
 #include <cooperative_groups.h>
 
 #include "api.h"

@@ -16,9 +16,11 @@
 // whole number of rows of vectors apart), each of the `top` best is searched for. Looking for candidates on the way instead (against a
 // bound from the first chunk) cost more: every candidate sends its warp on a detour.
 //
-// Bound by memory, closely followed by the exponentials (16 a cycle and SM: 14.5 us for 509 x 128256, whose bf16 logits take 19.9 to
-// read) and the other 5 instructions per element, for which additions and products are done in pairs; all rows of such a call end at
-// the same time, so the way from the last logit to the result (joining, the search among groups) is not hidden. Measured, back to back
+// Memory (19.9 us for 509 x 128256 bf16 logits), the exponentials (16 a cycle and SM: 14.5 us) and the other 5 instructions per element, for
+// which additions and products are done in pairs, come close to one another; no unit is at its limit (top 5: exponentials 41 %, issue 61 %,
+// memory 38 % busy), and 509 CTAs are four on some SMs and three on others. The way from the last logit to the result (joining, the search
+// among groups) leaves a CTA without loads on their way: top 5 of 2000 x 32000, whose rows have no common end, takes 55 us in place of 32.
+// Measured, back to back
 // (us): 509 x 128256 bf16 31 without alternatives (24.6 without the exponentials), 45 with top 5, 53 with top 20; 512 x 151936 fp32 55
 // (floor 47), 80, 107; one row of 151936 fp32 5.5, 10.2, 12.9.
 #include <cooperative_groups.h>
@@ -382,7 +384,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
 }
 
 // A row is cut while all CTAs still find an SM of their own, into parts of at least a chunk: with more CTAs the tails of the parts cost
-// more than the cut gives (74 rows of 128256 fp32, top 5: 16.5 us in 2 parts, 21.2 in 4; one row: 10.2 us in 8 parts, 22.9 in one).
+// more than the cut gives (74 rows of 128256 fp32, top 5: 16.5 us in 2 parts, 21.2 in 4; one row: 10.2 us in 8 parts, 22.9 in one). In
+// between it is not the best cut, as four CTAs fit on an SM and one alone does not fill it (us without alternatives / top 5 / top 20,
+// 128256 bf16): 200 rows 22.2 / 29.6 / 32.8 in one part, which the rule takes, 18.3 / 27.6 / 30.2 in two; 32 rows 9.5 / 16.8 / 18.4 in four,
+// which it takes, 8.7 / 14.6 / 16.5 in two.
 template <typename T, bool TOP>
 static cudaError_t launch_token_logprobs(const LpParams& p, int rows, cudaStream_t stream) {
   constexpr int THREADS = 256, chunk = THREADS * kLpVecs * 16 / sizeof(T);

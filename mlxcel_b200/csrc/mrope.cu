@@ -471,7 +471,8 @@ __global__ void __launch_bounds__(kMropeThreads, W == 8 ? 3 : 4) axial_rope_vec_
   }
 }
 
-// Tokens of a CTA: as many as have an angle per thread, while every SM still gets four CTAs.
+// Tokens of a CTA: as many as have an angle per thread, while every SM still gets four CTAs. Between 600 and 1200 tokens that is one a CTA
+// and more CTAs than are resident (1031 on 592 places: 8.1 us, of which a copy of the bytes takes 2.9).
 static int mrope_tokens(int T) {
   int n = kMropeTokens;
   while (n > 1 && T < 4 * n * device_sm_count()) n /= 2;
@@ -508,7 +509,9 @@ extern "C" int mx_mrope_append(const MxMropeAppend* a, void* stream_) {
   cudaError_t e;
   auto bits_of = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
   // Accesses of 8 bytes leave room for more warps, those of 16 bytes take fewer instructions: 1031 tokens of 32 + 4 heads 8.1 us against 10.8,
-  // 8191 of 64 + 16 heads with norms 81 against 73. Codes are made of 8 values of a lane at once.
+  // 8191 of 64 + 16 heads with norms 81 against 73. Codes are made of 8 values of a lane at once; each takes a
+  // division, and the 12 forms that make them spill 4 to 24 bytes (8191 tokens of 64 + 16 heads without norms 82 us with 8 bits, 80 with 4, 66
+  // with 16; 4000 of 32 + 16 heads 34, 33, 23).
   const bool coded = kv_bits != 16;
   int w = mrope_width(coded || mrope_tokens(T) == kMropeTokens ? 8 : 4, D, rot_dim, bits_of(a->qkv) | bits_of(a->q_out) | bits_of(a->q_norm_w) | bits_of(a->k_norm_w) |
                       (coded ? 0 : bits_of(a->k_pool) | bits_of(a->v_pool)), a->ldqkv | a->ldq);

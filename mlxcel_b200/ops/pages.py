@@ -1,4 +1,4 @@
-"""Pages of a cache on the move: copies between pages of a pool (copy on write, forks, compaction), pages gathered into one buffer
+"""Pages of a cache on the move: copies between pages of a pool, pages gathered into one buffer
 (snapshots, hand-off) and scattered from one (``csrc/pages.cu``; tables from ``host/page_plan.cpp``). A page id addresses the same
 slot of every slab, and every call moves all of a page in one launch per 128 slabs."""
 from __future__ import annotations
@@ -18,9 +18,9 @@ def _list(ids) -> list:
 
 
 class PageSlabs:
-    """The slabs of a pool, [pages, ...] each, apart in memory, in the order in which a buffer holds them. Page ids are host lists (or CPU tensors and
-    arrays) and are checked: a page outside the pool, a destination named twice or a source missing raises ``ValueError`` and moves
-    nothing. Slabs whose pages are empty are left out. The ids of small calls (106 copies, 320 pages) travel with the launch, which can
+    """The slabs of a pool, [pages, ...] each, apart in memory, in the order in which a buffer holds them. Page ids are host lists (or
+    CPU tensors and arrays) and are checked: a page outside the pool, a destination of two sources or a source missing raises ``ValueError``
+    and moves nothing. Slabs whose pages are empty are left out. The ids of small calls (106 copies, 320 pages) travel with the launch, which can
     be captured into a graph; longer tables are copied to the device first, which cannot."""
 
     def __init__(self, slabs: list[torch.Tensor]):
