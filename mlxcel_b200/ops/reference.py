@@ -254,7 +254,7 @@ def axial_rope(qkv, positions, inv_freq, axes, heads: int, D: int):
 
 def turned_heads(qkv, cos, sin, heads: int):
     """:func:`axial_rope` with the angles of :func:`axes_angles` (one forward's, for all its blocks), as views of any order."""
-    q, k, v = qkv.view(qkv.shape[0], 3, heads, -1).unbind(1)
+    q, k, v = qkv.view(qkv.shape[0], 3, heads, 2 * cos.shape[1]).unbind(1)
     return turn_heads(q, cos, sin).transpose(0, 1), turn_heads(k, cos, sin).transpose(0, 1), v.float().transpose(0, 1)
 
 

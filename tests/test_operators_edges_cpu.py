@@ -46,6 +46,12 @@ def test_mrope_entry_refuses_no_heads_before_it_launches():
     assert len(args) == struct.calcsize(rotary._ARGS.format) and _lib.load().mx_mrope_append(args, None) == -1
 
 
+@pytest.mark.parametrize("rows,heads", [(0, 2), (3, 0), (0, 0)])
+def test_axial_rope_of_nothing(rows, heads):
+    got = rotary.axial_rope(torch.zeros(rows, 3 * heads * 8), torch.zeros(2, rows, dtype=torch.int32), torch.ones(4), torch.zeros(4, dtype=torch.int32), heads=heads, D=8)
+    assert [t.shape for t in got] == [(heads, rows, 8)] * 3
+
+
 # ----------------------------------------------------------------------------- pages of the pool
 def test_slabs_that_share_memory_are_refused():
     """A chain of copies would be taken once per slab: pages 0, 1, 2 in place of 0, 0, 1 became 0, 0, 0."""
