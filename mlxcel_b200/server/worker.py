@@ -165,7 +165,14 @@ class ModelWorker:
 
         fut: concurrent.futures.Future = concurrent.futures.Future()
         self.inbox.put(("call", (fn, fut, name, tuple(args))))
-        return fut.result()
+        while True:
+            try:
+                return fut.result(timeout=1.0)
+            except TimeoutError:
+                if fut.done():                      # (the call's own)
+                    raise
+                if not self.thread.is_alive():      # nobody will make the call
+                    raise RuntimeError("the model's worker has ended") from None
 
     def _call_cache_reset(self):
         return self.engine.bm.reset_prefix_cache()

@@ -338,6 +338,21 @@ def test_echo_scores_between_steps_of_the_engine(client, monkeypatch):
     assert len(threads) >= 4 and len(set(threads)) == 1
 
 
+def test_echo_behind_the_end_of_the_worker():
+    """A worker that has ended makes no more calls: the request is answered with an error instead of waiting for it."""
+    cfg, tk = preset("tiny-llama"), ByteTokenizer(preset("tiny-llama").vocab_size)
+    eng = Engine(DecoderModel(cfg, random_weights(cfg, seed=0, dtype=torch.float32, std=0.05)), cfg, EngineConfig(num_blocks=32, max_model_len=128, cuda_graphs=False))
+    worker = ModelWorker(eng, tk, "tiny")
+    with TestClient(create_app(ServerState(worker, tk, "tiny"))) as c:
+        def late():
+            raise TimeoutError("its own")
+        with pytest.raises(TimeoutError, match="its own"):
+            worker.run_exclusive(late)
+        worker.shutdown()
+        r = c.post("/v1/completions", json={"prompt": "hello", "max_tokens": 0, "echo": True, "logprobs": True})
+        assert r.status_code == 400 and "ended" in r.text
+
+
 def test_a_number_of_log_probabilities_gives_alternatives_without_echo_too(client):
     got, want = _complete(client, logprobs=3), _complete(client, logprobs=True, top_logprobs=3)
     assert got == want and len(got["top_logprobs"]) == 3 and all(got["top_logprobs"])
