@@ -281,25 +281,37 @@ def token_logprobs(logits, ids, top: int = 0, bias=None, scale: float = 1.0, sof
     z = logits.float()
     if bias is not None:
         z = z + bias.float()
-    z = z * scale
+    if scale != 1.0:
+        z = z * scale
     if softcap > 0:
         z = softcap * torch.tanh(z / softcap)
-    z = torch.where(z.isnan(), torch.full_like(z, float("-inf")), z)
     m = z.amax(-1, keepdim=True)
+    if m.isnan().any():
+        z = torch.where(z.isnan(), torch.full_like(z, float("-inf")), z)
+        m = z.amax(-1, keepdim=True)
     # a logit of +inf takes all the mass (shared with its equals); equal infinities are at distance 0
-    gap = torch.where(z == m, torch.zeros_like(z), z - m)
-    e = torch.where(z == float("-inf"), torch.zeros_like(z), gap.exp())
-    s = e.sum(-1)
+    gap = torch.where(z == m, torch.zeros_like(z), z - m) if m.isinf().any() else z - m
+    gap.clamp_(min=-200.0)                                   # (e^-200 is no number of fp32: 0, also for masked ones)
+    e = gap.exp()
+    gone = m[:, 0] == float("-inf")
+    s = torch.where(gone, torch.zeros_like(gap[:, 0]), e.sum(-1))
     log_s = s.log()
-    gone = s == 0
-    lse = torch.where(gone, torch.full_like(s, float("-inf")), m[:, 0] + log_s)
-    entropy = torch.where(gone, torch.zeros_like(s), log_s - torch.where(e > 0, e * gap, torch.zeros_like(e)).sum(-1) / s)
-    logp = torch.where(z == float("-inf"), z, gap - log_s[:, None])
+    lse = torch.where(gone, m[:, 0], m[:, 0] + log_s)
+    entropy = torch.where(gone, torch.zeros_like(s), log_s - (e * gap).sum(-1) / s)
+
+    def logp(at):
+        x = z.gather(1, at)
+        return torch.where(x == float("-inf"), x, torch.where(x == m, torch.zeros_like(x), x - m) - log_s[:, None])
     V = z.shape[1]
     i2 = (ids if ids.dim() == 2 else ids[:, None]).long()
-    logprob = torch.where((i2 < 0) | (i2 >= V), torch.full_like(i2, float("nan"), dtype=torch.float32), logp.gather(1, i2.clamp(0, V - 1)))
-    order = torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :top]
-    return logprob.view(ids.shape), entropy, lse, order.int(), logp.gather(1, order)
+    logprob = torch.where((i2 < 0) | (i2 >= V), torch.full_like(i2, float("nan"), dtype=torch.float32), logp(i2.clamp(0, V - 1)))
+    order = i2[:, :0]
+    if top:
+        # (value, then lower index) as one number: the bits of a float in the order of its value, and the index from the end
+        bits = (z + 0.0).view(torch.int32)
+        key = (torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits).long() << 32) + (V - 1 - torch.arange(V, device=z.device))
+        order = V - 1 - (key.topk(top, -1).values & 0xFFFFFFFF)
+    return logprob.view(ids.shape), entropy, lse, order.int(), logp(order)
 
 
 def head_rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:

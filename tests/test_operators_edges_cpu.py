@@ -23,7 +23,7 @@ from mlxcel_b200.models.decoder import DecoderModel, StepBatch
 from mlxcel_b200.models.depth_anything import Dinov2Backbone
 from mlxcel_b200.models.weights import random_weights
 from mlxcel_b200.multimodal.qwen2_vision import Glm4vVisionTower, Qwen2VisionTower
-from mlxcel_b200.ops import KVLayer, _lib, pages, rotary
+from mlxcel_b200.ops import KVLayer, _lib, logprobs, pages, rotary
 from mlxcel_b200.server.app import ServerState, create_app
 from mlxcel_b200.server.worker import ModelWorker
 from mlxcel_b200.tokenizer import ByteTokenizer
@@ -265,6 +265,27 @@ def test_scores_with_a_head_or_bias_of_another_type():
             model.w.extra["lm_head_b"] = (torch.randn(cfg.vocab_size, generator=torch.Generator().manual_seed(1)) * 0.5).to(torch.bfloat16).to(bias)
         want = torch.log_softmax(model.logits(prefill_hidden(model, cfg, ids, 8), torch.arange(29)).double(), -1).gather(1, torch.tensor(ids[1:])[:, None])[:, 0]
         assert torch.allclose(sequence_scores(model, cfg, ids, 8).logprob.double(), want, atol=1e-4), (head, bias)
+
+
+def test_log_probabilities_alone_order_no_vocabulary(monkeypatch):
+    """Sorting every row costs thirty times what its log softmax does; alternatives come without it too, ties by index."""
+    x = torch.randn(6, 3001, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).float() * 3
+    x[1, 7:], x[2], x[3, 5], x[4, 100], x[5] = float("-inf"), float("-inf"), float("nan"), float("inf"), torch.finfo(torch.float32).min
+    x[0, ::2], x[0, 1::2] = 0.0, -0.0
+    z = torch.where(x.isnan(), torch.full_like(x, float("-inf")), x)
+    want = torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :64]
+    ids = torch.randint(0, 3001, (6, 4), generator=torch.Generator().manual_seed(2))
+
+    def never(*a, **k):
+        raise AssertionError("a vocabulary was sorted")
+    for name in ("sort", "argsort"):
+        monkeypatch.setattr(torch, name, never)
+        monkeypatch.setattr(torch.Tensor, name, never)
+    r, alone = logprobs.token_logprobs(x, ids, top=64), logprobs.token_logprobs(x, ids)
+    assert torch.equal(r.top_ids.long(), want) and alone.top_ids.shape == (6, 0)
+    assert all(torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0)) for a, b in zip(r[:3], alone[:3]))
+    assert torch.allclose(r.top_logprobs[5], torch.full((64,), -math.log(3001)), atol=1e-5) and r.top_logprobs[4, 0] == 0
+    assert (r.top_logprobs[1, 7:] == float("-inf")).all() and (r.top_logprobs[2] == float("-inf")).all() and r.entropy[2] == 0
 
 
 def test_alternatives_change_no_draw():
